@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define VMO_ABI_VERSION 13
+#define VMO_ABI_VERSION 14
 
 enum {
   VMO_OK = 0,
@@ -317,6 +317,90 @@ int vmo_lstep_bwd(const vmo_lstep_bwd_args* args, void* stream);
 /* vmo_lstep_bwd, with `delta` also from the last step of the multi-block grids (m <= 128 and head dims 16 / 32 / 64 /
  * 128); their other steps and the general kernel's shapes reject it. */
 int vmo_lstep_bwd_delta(const vmo_lstep_bwd_args* args, void* stream);
+
+/*
+ * Packed causal attention with grouped heads (no counterpart in the reference).
+ *
+ * Sequences of different lengths lie one behind the other: sequence s has query rows [q_offsets[s], q_offsets[s + 1]) and
+ * keys [k_offsets[s], k_offsets[s + 1]).  With past = keys - queries of it, its row i attends to its keys j <= i + past
+ * (causal != 0) or to all of them; `heads` query heads, key / value head h / (heads / kv_heads) serves head h.
+ *
+ *   o[h, i, :] = sum_j softmax_j(sm_scale q_i . k_j) v_j     (0 for a row without keys)
+ *
+ * Views: stride_b is not used; q, o, grad_o, grad_q (heads, tq, d), the others (kv_heads, tk, d).  d is 64 or 128.  The
+ * offsets (n + 1 int32 each, not falling) are read on the GPU and cut to [0, tq] and [0, tk]; n is at most 2048.  lse:
+ * (heads, tq) fp32, log2 units, rows stat_stride apart (the forward's output, may be null there; the backward's input).
+ * zero_rest: rows of o outside every sequence are written as zeros (else they are left as they were); the backward always
+ * writes zeros to such rows of its gradients.
+ */
+enum { VMO_PACKED_MAX_SEQUENCES = 2048 };
+typedef struct vmo_packed_args {
+  int32_t dtype, heads, kv_heads, n, tq, tk, d, causal, zero_rest;
+  vmo_view q, k, v, o;
+  const int32_t *q_offsets, *k_offsets;
+  float* lse;
+  int64_t stat_stride;
+  float sm_scale;
+  /* backward only */
+  vmo_view grad_o, grad_q, grad_k, grad_v;
+  void* workspace;
+  size_t workspace_bytes;
+} vmo_packed_args;
+
+int vmo_packed_fwd(const vmo_packed_args* args, void* stream);
+size_t vmo_packed_bwd_workspace_size(const vmo_packed_args* args);
+int vmo_packed_bwd(const vmo_packed_args* args, void* stream);
+
+/*
+ * Attention of one new token a sequence over a paged key / value cache (no counterpart in the reference).
+ *
+ * Pages are (pages, kv_heads, page_size, d) views (k, v: stride_b from page to page); token t of sequence b lies at place
+ * t % page_size of page table[b * table_stride + t / page_size].  q, o: (batch, heads, d), stride_b and stride_h used.
+ *   o[b, h, :] = sum_t softmax_t(sm_scale q . k_t) v_t,  t < lengths[b]     (0 for a length of 0)
+ * The table and the lengths are read on the GPU.  A page number outside [0, pages), or a length beyond the table's width,
+ * is not followed: that sequence's rows of o are NaN.  page_size: a power of two from 8 to 1024; d is 64 or 128.
+ */
+typedef struct vmo_paged_args {
+  int32_t dtype, batch, heads, kv_heads, d, pages, page_size, table_width;
+  vmo_view q, k, v, o;
+  const int32_t *table, *lengths;
+  int64_t table_stride;
+  float sm_scale;
+  void* workspace;
+  size_t workspace_bytes;
+} vmo_paged_args;
+
+size_t vmo_paged_attention_workspace_size(const vmo_paged_args* args);
+int vmo_paged_attention(const vmo_paged_args* args, void* stream);
+
+/*
+ * New key and value rows into a paged cache: k, v are (kv_heads, tokens, d) views (stride_b not used), sequence b's rows
+ * are [offsets[b], offsets[b + 1]) -- or row b alone where offsets is null -- and its last one goes to token
+ * lengths[b] - 1, the others before it.  A row of no sequence, or one whose page number or place is outside, is left out.
+ * 16-bit elements; d a multiple of 8.
+ */
+typedef struct vmo_append_args {
+  int32_t sequences, tokens, kv_heads, d, pages, page_size, table_width;
+  vmo_view k, v, k_pages, v_pages;
+  const int32_t *table, *lengths, *offsets;
+  int64_t table_stride;
+} vmo_append_args;
+
+int vmo_append_pages(const vmo_append_args* args, void* stream);
+
+/*
+ * Pages copied within a cache: page src[i] to page dst[i], in each of `layers` layers (layer_bytes apart) of k and of v.
+ * A page is page_bytes together.  src and dst are host arrays, read before the call returns; a page that is written twice,
+ * or written and read, is refused.
+ */
+typedef struct vmo_copy_args {
+  int32_t layers, pages, pairs;
+  void *k, *v;
+  int64_t page_bytes, layer_bytes;
+  const int32_t *src, *dst;
+} vmo_copy_args;
+
+int vmo_copy_pages(const vmo_copy_args* args, void* stream);
 
 #ifdef __cplusplus
 }

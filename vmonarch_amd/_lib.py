@@ -13,7 +13,7 @@ import threading
 import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libvmonarch_gfx950.so")
-ABI_VERSION = 13
+ABI_VERSION = 14
 FEA_FWD_SCRATCH_BYTES = 32 << 20   # VMO_FEA_FWD_SCRATCH_BYTES: scratch of vmo_fea_fwd_noalloc per GPU
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
@@ -78,6 +78,40 @@ class LstepBwdArgs(ctypes.Structure):
     ]
 
 
+class PackedArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("heads", c_int32), ("kv_heads", c_int32), ("n", c_int32), ("tq", c_int32), ("tk", c_int32),
+        ("d", c_int32), ("causal", c_int32), ("zero_rest", c_int32), ("q", View), ("k", View), ("v", View), ("o", View),
+        ("q_offsets", c_void_p), ("k_offsets", c_void_p), ("lse", c_void_p), ("stat_stride", c_int64), ("sm_scale", c_float),
+        ("grad_o", View), ("grad_q", View), ("grad_k", View), ("grad_v", View), ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
+class PagedArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("batch", c_int32), ("heads", c_int32), ("kv_heads", c_int32), ("d", c_int32), ("pages", c_int32),
+        ("page_size", c_int32), ("table_width", c_int32), ("q", View), ("k", View), ("v", View), ("o", View),
+        ("table", c_void_p), ("lengths", c_void_p), ("table_stride", c_int64), ("sm_scale", c_float), ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("sequences", c_int32), ("tokens", c_int32), ("kv_heads", c_int32), ("d", c_int32), ("pages", c_int32),
+        ("page_size", c_int32), ("table_width", c_int32), ("k", View), ("v", View), ("k_pages", View), ("v_pages", View),
+        ("table", c_void_p), ("lengths", c_void_p), ("offsets", c_void_p), ("table_stride", c_int64),
+    ]
+
+
+class CopyArgs(ctypes.Structure):
+    _fields_ = [
+        ("layers", c_int32), ("pages", c_int32), ("pairs", c_int32), ("k", c_void_p), ("v", c_void_p), ("page_bytes", c_int64),
+        ("layer_bytes", c_int64), ("src", c_void_p), ("dst", c_void_p),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -111,6 +145,13 @@ def lib():
         L.vmo_fea_bwd_workspace_size.argtypes = [ctypes.POINTER(FeaBwdArgs)]
         L.vmo_fea_bwd.restype = ctypes.c_int
         L.vmo_fea_bwd.argtypes = [ctypes.POINTER(FeaBwdArgs), c_void_p]
+        L.vmo_packed_bwd_workspace_size.restype = L.vmo_paged_attention_workspace_size.restype = c_size_t
+        L.vmo_packed_bwd_workspace_size.argtypes = [ctypes.POINTER(PackedArgs)]
+        L.vmo_paged_attention_workspace_size.argtypes = [ctypes.POINTER(PagedArgs)]
+        for name, args in (("vmo_packed_fwd", PackedArgs), ("vmo_packed_bwd", PackedArgs), ("vmo_paged_attention", PagedArgs),
+                           ("vmo_append_pages", AppendArgs), ("vmo_copy_pages", CopyArgs)):
+            f = getattr(L, name)
+            f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(args), c_void_p]
         v = L.vmo_abi_version()
         if v != ABI_VERSION:
             raise RuntimeError(f"vmonarch_amd: library ABI {v}, bindings expect {ABI_VERSION}")

@@ -17,7 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libvmonarch_gfx950.so")
-SOURCES = ["capi.hip", "fea_fwd.hip", "fea_fwd_ks.hip", "fea_bwd.hip", "lstep.hip", "lstep_mb.hip"]
+SOURCES = ["capi.hip", "fea_fwd.hip", "fea_fwd_ks.hip", "fea_bwd.hip", "lstep.hip", "lstep_mb.hip",
+           "packed.hip", "packed_fwd.hip", "packed_bwd.hip", "paged.hip"]
 HOST_LIB = os.path.join(HERE, "_vmo_host.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
@@ -28,6 +29,13 @@ FLAGS = [
     "-mno-amdgpu-ieee", "-fno-honor-nans",
     "-I", os.path.join(os.path.dirname(HERE), "include"),
 ]
+
+# Sources whose inputs may hold infinities and NaN where a mask hides them: compiled without the two flags above.
+NAN_SOURCES = {"packed.hip", "packed_fwd.hip", "packed_bwd.hip", "paged.hip"}
+
+
+def _flags(source):
+    return [f for f in FLAGS if source not in NAN_SOURCES or f not in ("-mno-amdgpu-ieee", "-fno-honor-nans")]
 
 
 def _run(cmd):
@@ -53,7 +61,7 @@ def build(verbose=False, jobs=None):
     os.makedirs(BUILD, exist_ok=True)
     srcs = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
     objs = [os.path.join(BUILD, os.path.splitext(s)[0] + ".o") for s in srcs]
-    cmds = [[HIPCC, *FLAGS, "-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(srcs, objs)]
+    cmds = [[HIPCC, *_flags(s), "-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(srcs, objs)]
     with ThreadPoolExecutor(max_workers=jobs or min(8, len(cmds))) as ex:
         for out in ex.map(_run, cmds):
             if verbose and out.strip():

@@ -583,6 +583,205 @@ std::tuple<Tensor, Tensor, Tensor> vmonarch_bwd(const std::vector<int>& orders, 
   return {gq, gk, gv};
 }
 
+// ---- packed prompts and the paged cache -------------------------------------------------------------------------
+// Shapes, types and devices are all checked before the first launch.  Tensors are (heads, tokens, D); inputs whose rows
+// the kernels cannot read in place are copied, tensors that are written are refused instead.
+
+bool rows_ok(const Tensor& t) {   // 16-byte aligned rows, one behind the other, contiguous features
+  const int64_t n = t.dim();
+  if (t.stride(n - 1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || t.stride(n - 2) <= 0) return false;
+  for (int64_t d = 0; d < n - 1; ++d)
+    if (t.stride(d) % 8) return false;
+  return true;
+}
+Tensor readable(const Tensor& t) { return rows_ok(t) ? t : t.contiguous(); }
+void writable(const Tensor& t, const char* msg) {
+  if (t.numel() == 0) return;
+  bool ok = rows_ok(t);
+  for (int64_t d = 0; d < t.dim(); ++d) ok = ok && (t.size(d) == 1 || t.stride(d) > 0);
+  if (!ok) throw py::value_error(msg);
+}
+vmo_view rows_view(const Tensor& t) { return vmo_view{t.data_ptr(), 0, t.stride(0), t.stride(1)}; }   // (heads, tokens, D)
+vmo_view pages_view(const Tensor& t) { return vmo_view{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+// an uninitialised tensor in the memory order of ref's (heads, tokens)
+Tensor empty_rows(const Tensor& ref) {
+  const int64_t H = ref.size(0), N = ref.size(1), D = ref.size(2);
+  return ref.stride(0) >= ref.stride(1) ? at::empty({H, N, D}, ref.options()) : at::empty({N, H, D}, ref.options()).transpose(0, 1);
+}
+int32_t size32(int64_t n) {
+  if (n > (1ll << 30)) throw py::value_error("vmonarch_amd: a size is above 2^30");
+  return (int32_t)n;
+}
+void index_list(const Tensor& q, const Tensor& t, int64_t dims, const char* msg) {
+  require(t.dim() == dims && t.scalar_type() == at::kInt && (t.numel() == 0 || t.stride(dims - 1) == 1), msg);
+  same_device(q, t);
+}
+
+vmo_packed_args packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_off, const Tensor& k_off,
+                            double sm_scale, bool causal) {
+  vmo_packed_args a{};
+  a.dtype = dtype_code(q);
+  a.heads = size32(q.size(0)); a.kv_heads = size32(k.size(0)); a.n = size32(q_off.size(0) - 1);
+  a.tq = size32(q.size(1)); a.tk = size32(k.size(1)); a.d = size32(q.size(2)); a.causal = causal;
+  a.q = rows_view(q); a.k = rows_view(k); a.v = rows_view(v);
+  a.q_offsets = q_off.data_ptr<int32_t>(); a.k_offsets = k_off.data_ptr<int32_t>();
+  a.sm_scale = (float)sm_scale;
+  return a;
+}
+void packed_checks(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_off, const Tensor& k_off) {
+  require(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k and v are (heads, tokens, D)");
+  like(q, {&k, &v});
+  require(k.sizes() == v.sizes() && q.size(2) == k.size(2), "k and v of one shape, q with their head dim");
+  require(k.size(0) > 0 && q.size(0) > 0 && q.size(0) % k.size(0) == 0, "query heads are a multiple of the key / value heads");
+  for (const Tensor* t : {&q_off, &k_off}) index_list(q, *t, 1, "offsets are int32, one-dimensional, on q's GPU");
+  require(q_off.size(0) >= 1 && q_off.size(0) == k_off.size(0), "offsets: one more than the sequences, as many for keys as for queries");
+}
+
+std::tuple<Tensor, OptT> packed_fwd(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& q_off,
+                                    const Tensor& k_off, double sm_scale, bool causal, const OptT& out, bool want_lse) {
+  packed_checks(q_in, k_in, v_in, q_off, k_off);
+  if (out) {
+    like(q_in, *out);
+    require(out->sizes() == q_in.sizes(), "out is shaped like q");
+    writable(*out, "vmonarch_amd: out needs 16-byte aligned rows with contiguous features");
+  }
+  const OnGpuOf device(q_in);
+  const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
+  vmo_packed_args a = packed_args(q, k, v, q_off, k_off, sm_scale, causal);
+  const Tensor o = out ? *out : empty_rows(q);
+  OptT lse;
+  if (want_lse) {
+    lse = at::empty({q.size(0), q.size(1)}, f32(q));
+    a.lse = lse->data_ptr<float>();
+    a.stat_stride = q.size(1);
+  }
+  a.o = rows_view(o);
+  a.zero_rest = !out;
+  check(vmo_packed_fwd(&a, stream_of(q)), "vmo_packed_fwd");
+  return {o, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> packed_bwd(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o_in,
+                                              const Tensor& lse, const Tensor& dO_in, const Tensor& q_off, const Tensor& k_off,
+                                              double sm_scale, bool causal) {
+  packed_checks(q_in, k_in, v_in, q_off, k_off);
+  like(q_in, {&o_in, &dO_in});
+  same_device(q_in, lse);
+  require(o_in.sizes() == q_in.sizes() && dO_in.sizes() == q_in.sizes(), "o and its gradient are shaped like q");
+  require(lse.dim() == 2 && lse.size(0) == q_in.size(0) && lse.size(1) == q_in.size(1) && lse.is_contiguous() &&
+              lse.scalar_type() == at::kFloat, "lse is the forward's");
+  const OnGpuOf device(q_in);
+  const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in), o = readable(o_in), dO = readable(dO_in);
+  vmo_packed_args a = packed_args(q, k, v, q_off, k_off, sm_scale, causal);
+  const Tensor dq = empty_rows(q_in), dk = empty_rows(k_in), dv = empty_rows(v_in);
+  a.o = rows_view(o); a.grad_o = rows_view(dO);
+  a.grad_q = rows_view(dq); a.grad_k = rows_view(dk); a.grad_v = rows_view(dv);
+  a.lse = lse.data_ptr<float>();
+  a.stat_stride = lse.size(1);
+  const Tensor ws = workspace(vmo_packed_bwd_workspace_size(&a), q);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = ws.numel();
+  check(vmo_packed_bwd(&a, stream_of(q)), "vmo_packed_bwd");
+  return {dq, dk, dv};
+}
+
+void cache_checks(const Tensor& x, const Tensor& k_pages, const Tensor& v_pages) {
+  require(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), "k_pages and v_pages are (pages, heads, page tokens, D)");
+  like(x, {&k_pages, &v_pages});
+}
+
+Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
+                       double sm_scale, const OptT& out) {
+  require(q_in.dim() == 3, "q is (sequences, heads, D)");
+  cache_checks(q_in, k_pages, v_pages);
+  require(q_in.size(2) == k_pages.size(3), "q has the cache's head dim");
+  require(k_pages.size(1) > 0 && q_in.size(1) > 0 && q_in.size(1) % k_pages.size(1) == 0,
+          "query heads are a multiple of the key / value heads");
+  index_list(q_in, table, 2, "the page table is int32, (sequences, page numbers), on q's GPU");
+  index_list(q_in, lengths, 1, "lengths are int32, one-dimensional, on q's GPU");
+  require(table.size(0) == q_in.size(0) && lengths.size(0) == q_in.size(0), "one row of the page table and one length a sequence");
+  if (out) {
+    like(q_in, *out);
+    require(out->sizes() == q_in.sizes(), "out is shaped like q");
+    writable(*out, "vmonarch_amd: out needs 16-byte aligned rows with contiguous features");
+  }
+  const OnGpuOf device(q_in);
+  const Tensor q = readable(q_in), o = out ? *out : at::empty(q_in.sizes(), q_in.options());
+  vmo_paged_args a{};
+  a.dtype = dtype_code(q);
+  a.batch = size32(q.size(0)); a.heads = size32(q.size(1)); a.kv_heads = size32(k_pages.size(1)); a.d = size32(q.size(2));
+  a.pages = size32(k_pages.size(0)); a.page_size = size32(k_pages.size(2)); a.table_width = size32(table.size(1));
+  a.q = vmo_view{q.data_ptr(), q.stride(0), q.stride(1), q.stride(1)};
+  a.o = vmo_view{o.data_ptr(), o.stride(0), o.stride(1), o.stride(1)};
+  a.k = pages_view(k_pages); a.v = pages_view(v_pages);
+  a.table = table.data_ptr<int32_t>(); a.lengths = lengths.data_ptr<int32_t>();
+  a.table_stride = table.stride(0);
+  a.sm_scale = (float)sm_scale;
+  Tensor ws;
+  if (const size_t bytes = vmo_paged_attention_workspace_size(&a)) {
+    ws = workspace(bytes, q);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  check(vmo_paged_attention(&a, stream_of(q)), "vmo_paged_attention");
+  return o;
+}
+
+void append_pages(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+                  const Tensor& lengths, const OptT& offsets) {
+  require(k_in.dim() == 3 && k_in.sizes() == v_in.sizes(), "k and v are (heads, tokens, D), of one shape");
+  dtype_code(k_in);
+  like(k_in, v_in);
+  cache_checks(k_in, k_pages, v_pages);
+  require(k_in.size(0) == k_pages.size(1) && k_in.size(2) == k_pages.size(3), "k and v have the cache's heads and head dim");
+  index_list(k_in, table, 2, "the page table is int32, (sequences, page numbers), on k's GPU");
+  index_list(k_in, lengths, 1, "lengths are int32, one-dimensional, on k's GPU");
+  require(table.size(0) == lengths.size(0), "one row of the page table and one length a sequence");
+  if (offsets) {
+    index_list(k_in, *offsets, 1, "offsets are int32, one-dimensional, on k's GPU");
+    require(offsets->size(0) == lengths.size(0) + 1, "offsets: one more than the sequences");
+  } else {
+    require(k_in.size(1) == lengths.size(0), "without offsets k and v hold one row a sequence");
+  }
+  for (const Tensor* t : {&k_pages, &v_pages}) writable(*t, "vmonarch_amd: pages need 16-byte aligned rows with contiguous features");
+  const OnGpuOf device(k_in);
+  const Tensor k = readable(k_in), v = readable(v_in);
+  vmo_append_args a{};
+  a.sequences = size32(lengths.size(0)); a.tokens = size32(k.size(1)); a.kv_heads = size32(k.size(0)); a.d = size32(k.size(2));
+  a.pages = size32(k_pages.size(0)); a.page_size = size32(k_pages.size(2)); a.table_width = size32(table.size(1));
+  a.k = rows_view(k); a.v = rows_view(v);
+  a.k_pages = pages_view(k_pages); a.v_pages = pages_view(v_pages);
+  a.table = table.data_ptr<int32_t>(); a.lengths = lengths.data_ptr<int32_t>();
+  a.offsets = offsets ? offsets->data_ptr<int32_t>() : nullptr;
+  a.table_stride = table.stride(0);
+  check(vmo_append_pages(&a, stream_of(k)), "vmo_append_pages");
+}
+
+void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const std::vector<int64_t>& src, const std::vector<int64_t>& dst) {
+  require((k_pages.dim() == 4 || k_pages.dim() == 5) && v_pages.sizes() == k_pages.sizes(),
+          "k_pages and v_pages are (pages, heads, page tokens, D), or (layers, pages, ..)");
+  require(k_pages.element_size() == 2, "16-bit pages");
+  like(k_pages, v_pages);
+  require(k_pages.is_contiguous() && v_pages.is_contiguous(), "contiguous k_pages and v_pages");
+  require(src.size() == dst.size(), "as many pages to copy as places to copy them to");
+  const int64_t at = k_pages.dim() - 4, pages = k_pages.size(at);
+  const OnGpuOf device(k_pages);
+  std::vector<int32_t> s, d;
+  for (size_t i = 0; i < src.size(); ++i) {
+    if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages)
+      throw py::value_error("vmonarch_amd: page " + std::to_string(src[i]) + " to " + std::to_string(dst[i]) + " of " + std::to_string(pages));
+    s.push_back((int32_t)src[i]);
+    d.push_back((int32_t)dst[i]);
+  }
+  vmo_copy_args a{};
+  a.layers = size32(at ? k_pages.size(0) : 1); a.pages = size32(pages); a.pairs = size32((int64_t)s.size());
+  a.k = k_pages.data_ptr(); a.v = v_pages.data_ptr();
+  a.page_bytes = k_pages.size(at + 1) * k_pages.size(at + 2) * k_pages.size(at + 3) * 2;
+  a.layer_bytes = pages * a.page_bytes;
+  a.src = s.data(); a.dst = d.data();
+  check(vmo_copy_pages(&a, stream_of(k_pages)), "vmo_copy_pages");
+}
+
 // A single launch as an entry of its own: on its first tensor's GPU.
 template <class R, class... A>
 auto on_its_gpu(R (*launch)(const Tensor&, A...)) {
@@ -609,6 +808,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
     const py::gil_scoped_release unlocked;
     return vmonarch_fwd(q, k, v, m, b, iters, recompute_tokens, min_col_mass, scale, qk_fp8, splits, overlap, side_handle, stage);
   });
+  mod.def("packed_fwd", &packed_fwd, NoGil());
+  mod.def("packed_bwd", &packed_bwd, NoGil());
+  mod.def("paged_attention", &paged_attention, NoGil());
+  mod.def("append_pages", &append_pages, NoGil());
+  mod.def("copy_pages", &copy_pages, NoGil());
   mod.def("vmonarch_fwd_train", &vmonarch_fwd_train, NoGil());
   mod.def("vmonarch_bwd", &vmonarch_bwd, NoGil());
 }

@@ -1,0 +1,236 @@
+// Packed causal attention: launch parameters, the order of its workgroups and what a masked block's products take, shared
+// by the forward (packed_fwd.hip) and the backward (packed_bwd.hip).
+//
+// Sequence s holds query rows [q_off[s], q_off[s + 1]) and keys [k_off[s], k_off[s + 1]) of the packed tensors.  With
+// past = nk - nq, its row i sees the keys j <= i + past (causal), or all of them.  The offsets are read on the GPU, so a
+// captured graph replays with others; they are cut to the tensors, so none reaches outside.
+#pragma once
+
+#include "fea_fwd.h"
+
+namespace vmo {
+
+constexpr int kPackedMaxSeqs = 2048;   // a call's sequences: their tile counts wait in LDS while a workgroup finds its tile
+constexpr int kPackedTile = 128;       // queries of a forward / dq workgroup, keys of a dk / dv one
+constexpr int kPackedWaves = 4;
+
+struct PackedParams {
+  const void *q, *k, *v, *o, *dO;
+  void *out, *dq, *dk, *dv;
+  int64_t q_sh, q_sn, k_sh, k_sn, v_sh, v_sn, o_sh, o_sn, do_sh, do_sn;
+  int64_t dq_sh, dq_sn, dk_sh, dk_sn, dv_sh, dv_sn;
+  const int32_t *q_off, *k_off;
+  int n, tq, tk, heads, kv_heads, group;   // group = heads / kv_heads
+  int causal, zero_rest;                   // zero_rest: rows outside every sequence are written as zeros
+  float* lse;                              // (heads, tq), log2 units, rows of st_sh
+  int64_t st_sh;
+  float* neg_delta;                        // (heads, tq): -rowsum(o dO), from the dq kernel to the dk / dv one
+  float *dk_part, *dv_part;                // (splits, kv_heads, tk, D) fp32 when the group's heads are split
+  int splits;                              // workgroups that share a key tile, each with group / splits of the heads
+  float c, sm_scale;                       // c = sm_scale log2 e
+};
+
+// ---- integer sums over a wave (DPP: row shifts, then the rows' last lanes broadcast) --------------------------------
+__device__ __forceinline__ int wave_scan_i32(int v) {   // inclusive prefix sum over the lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+__device__ __forceinline__ int wave_sum_i32(int v) { return __builtin_amdgcn_readlane(wave_scan_i32(v), 63); }
+
+// ---- which tile a workgroup takes ------------------------------------------------------------------------------------
+struct PackedSeq { int qb, nq, kb, nk; };
+
+__device__ __forceinline__ PackedSeq packed_seq(const PackedParams& p, int s) {
+  PackedSeq r;
+  r.qb = min(max(p.q_off[s], 0), p.tq);
+  r.nq = min(max(p.q_off[s + 1], r.qb), p.tq) - r.qb;
+  r.kb = min(max(p.k_off[s], 0), p.tk);
+  r.nk = min(max(p.k_off[s + 1], r.kb), p.tk) - r.kb;
+  return r;
+}
+
+// Tiles of a sequence in the order u = 0, 1, .. of falling work: u's work, in tiles of the other side, is
+// max(0, min(cap, top - u)).  Query tiles: a causal row's keys grow with it, so u counts from the last tile; key tiles: a
+// key's queries fall with it.
+struct PackedTiles { int tiles, top, cap; };
+template <bool KEYS>
+__device__ __forceinline__ PackedTiles packed_tiles(const PackedParams& p, const PackedSeq& s) {
+  constexpr int T = kPackedTile, kMany = 1 << 28;
+  const int qt = (s.nq + T - 1) / T, kt = (s.nk + T - 1) / T;
+  if constexpr (KEYS) return PackedTiles{kt, p.causal ? kt : kMany, qt};
+  return PackedTiles{qt, p.causal ? kt : kMany, kt};
+}
+// how many of a sequence's tiles have at least the work `level`
+__device__ __forceinline__ int packed_count(const PackedTiles& t, int level) {
+  if (level <= 0) return t.tiles;
+  return level <= t.cap ? min(max(t.top - level + 1, 0), t.tiles) : 0;
+}
+
+struct PackedTile {
+  int seq, tile;   // tile < 0: none; seq then numbers the spare workgroups from 0
+  int spare;       // how many there are
+};
+
+// The idx-th tile over all sequences, heaviest first (a tile's time is its keys, or queries: with the heavy ones first the
+// chip's last round is made of light ones).  The largest level that more than idx tiles reach is found by bisection over
+// per-sequence counts that lie in LDS (`lds`: 12 bytes a sequence, free again after the next barrier); a level holds the
+// sequences in order.  Every wave does the same; ~0.3 us for up to 64 sequences.
+template <bool KEYS>
+__device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int idx, int blocks, VMO_LDS int* lds) {
+  const int lane = threadIdx.x & 63;
+  int best = 0;
+  for (int s = threadIdx.x; s < p.n; s += 64 * kPackedWaves) {
+    const PackedTiles t = packed_tiles<KEYS>(p, packed_seq(p, s));
+    lds[3 * s] = t.tiles;
+    lds[3 * s + 1] = t.top;
+    lds[3 * s + 2] = t.cap;
+  }
+  __syncthreads();
+  auto at = [&](int s) __attribute__((always_inline)) { return PackedTiles{lds[3 * s], lds[3 * s + 1], lds[3 * s + 2]}; };
+  auto total = [&](int level) __attribute__((always_inline)) {
+    int c = 0;
+    for (int s = lane; s < p.n; s += 64) c += packed_count(at(s), level);
+    return wave_sum_i32(c);
+  };
+  for (int s = lane; s < p.n; s += 64) best = max(best, lds[3 * s] > 0 ? min(lds[3 * s + 1], lds[3 * s + 2]) : 0);
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) best = max(best, __shfl_xor(best, m));
+  PackedTile r;
+  const int all = total(0);
+  r.spare = blocks - all;
+  r.tile = -1;
+  r.seq = idx - all;
+  if (idx < all) {
+    int lo = 0, hi = __builtin_amdgcn_readfirstlane(best) + 1;   // total(lo) > idx >= total(hi) = 0
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (total(mid) > idx) lo = mid;
+      else hi = mid;
+    }
+    int left = idx - total(lo + 1);
+    for (int s0 = 0; s0 < p.n; s0 += 64) {
+      const int s = s0 + lane;
+      const PackedTiles t = s < p.n ? at(s) : PackedTiles{0, 0, 0};
+      const int before = packed_count(t, lo + 1), mine = packed_count(t, lo) - before;
+      const int upto = wave_scan_i32(mine), here = __builtin_amdgcn_readlane(upto, 63);
+      if (left < here) {
+        const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > left));
+        const int u = __builtin_amdgcn_readlane(before, who) + left -
+                      (__builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(mine, who));
+        r.seq = s0 + who;
+        r.tile = KEYS || !p.causal ? u : __builtin_amdgcn_readlane(t.tiles, who) - 1 - u;
+        break;
+      }
+      left -= here;
+    }
+  }
+  __syncthreads();   // every wave has read the counts
+  return r;
+}
+
+// Zeros for the rows outside every sequence, 128-row pieces dealt to the spare workgroups (there is one at least
+// whenever there is such a row: the grid has ceil(rows / 128) + n tiles).
+template <class T, int D>
+__device__ __forceinline__ void packed_zero_rest(T* rows, int64_t sn, const int32_t* off, int n, int total, int which,
+                                                 int spare) {
+  static_assert(sizeof(T) == 2, "16-bit rows");
+  constexpr int CH = D / 8;
+  const int first = min(max(off[0], 0), total), last = min(max(off[n], 0), total);
+  for (int r0 = which * kPackedTile; r0 < total; r0 += spare * kPackedTile)
+    for (int i = threadIdx.x; i < kPackedTile * CH; i += 64 * kPackedWaves) {
+      const int r = r0 + i / CH;
+      if (r < total && (r < first || r >= last)) *(uint4*)((char*)(rows + r * sn) + (i % CH) * 16) = uint4{0, 0, 0, 0};
+    }
+}
+
+// ---- products over a block with masked rows ---------------------------------------------------------------------------
+template <bool F16> constexpr uint32_t kInfBits = F16 ? 0x7c00u : 0x7f80u;   // from here on: an infinity or a NaN
+
+// acc[a] += W^T P for 32 rows W of an LDS tile (RB-byte rows, swizzled) and the packed weights P of the accumulator layout
+// (element e of P[h]: row 16 h + 8 (e / 4) + 4 hl + e % 4 of the lane's column).  Rows that the lane's column does not see
+// have weight 0, but 0 times an infinity or NaN is a NaN: where a wave's operands hold such values they are taken as 0,
+// and a second pass adds them to the columns that do see their row.
+template <bool F16, int RB, int NA, class Sees>
+__device__ __forceinline__ void masked_product(f32x16 (&acc)[NA], const VMO_LDS char* W, const typename Elem<F16>::V8 (&P)[2],
+                                               int lane, Sees sees) {
+  using E = Elem<F16>;
+  using T = typename E::T;
+  using V8 = typename E::V8;
+  using V4 = typename E::V4;
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+  const int hl = lane >> 5;
+  const int trow = 4 * hl + ((lane & 15) >> 2), tchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), tbyte = (lane & 1) * 8;
+  bool odd = false;
+#pragma unroll
+  for (int a = 0; a < NA; ++a) {
+    V8 w[2];
+    u16x2 big = {0, 0};
+    const int c0 = trow * RB + (((4 * a + tchunk) ^ swz_rows<RB>(trow)) * 16 + tbyte);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const VMO_LDS char* rp = W + 16 * h * RB;
+      w[h] = lds_read_tr8<V8>(rp + c0, rp + 8 * RB + (c0 ^ 32));
+      const u32x4 bits = __builtin_bit_cast(u32x4, w[h]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, bits[j] & 0x7fff7fffu));
+    }
+    if (__builtin_amdgcn_ballot_w64(max((uint32_t)big[0], (uint32_t)big[1]) >= kInfBits<F16>) != 0) {
+      odd = true;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u16x8 b = __builtin_bit_cast(u16x8, w[h]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = (b[e] & 0x7fff) >= kInfBits<F16> ? 0 : b[e];
+        w[h] = __builtin_bit_cast(V8, b);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) acc[a] = E::mfma(w[h], P[h], acc[a]);
+  }
+  if (odd) {
+#pragma unroll 1
+    for (int row = 0; row < 32; ++row) {
+      // the weight of `row`: register 4 (row / 8) + row % 4 of the half (row / 4) % 2
+      float x = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x = r == 4 * (row >> 3) + (row & 3) ? (float)P[r >> 3][r & 7] : x;
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      x = __uint_as_float((row >> 2) & 1 ? both[1] : both[0]);
+      const bool seen = sees(row);
+      const VMO_LDS char* wr = W + row * RB + 8 * hl;
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {   // features 32 a + 8 g + 4 hl .. + 3
+          const u16x4 b = *(const VMO_LDS u16x4*)(wr + ((4 * a + g) ^ swz_rows<RB>(row)) * 16);
+          const V4 f = __builtin_bit_cast(V4, b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = fmaf(x, (float)f[e], acc[a][4 * g + e]);
+            acc[a][4 * g + e] = seen && (b[e] & 0x7fff) >= kInfBits<F16> ? y : acc[a][4 * g + e];
+          }
+        }
+    }
+  }
+}
+
+// Head of position `pos` among the workgroups of one tile: block b runs on XCD b % 8, so with g = gcd(8, heads) the
+// positions of one residue mod g stay on 8 / g XCDs; they take neighbouring heads, whose keys and values are shared.
+__device__ __forceinline__ int packed_head(int pos, int heads) {
+  const int g = heads & 7 ? (heads & 3 ? (heads & 1 ? 1 : 2) : 4) : 8;
+  return (pos % g) * (heads / g) + pos / g;
+}
+
+int packed_fwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);
+int packed_bwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);
+int packed_bwd_splits(int64_t tk, int n, int kv_heads, int group);
+
+}  // namespace vmo

@@ -1,0 +1,455 @@
+// Packed causal attention, backward.  With P from the saved row statistics (log2 units, P = 2^(s c - lse)):
+//   delta_i = sum_d o_id dO_id,  dP = dO V^T,  dS = P (dP - delta),  dQ = sm_scale dS K,  dK = sm_scale dS^T Q,
+//   dV = P^T dO, dK and dV summed over the query heads that share the key / value head.
+//
+// Two kernels, as the flash-entropy backward has them (no atomics, so a gradient's bits do not depend on timing):
+//  * packed_bwd_dq: 128 queries of one head, 32 a wave, one a lane; S^T = K Q^T and dP^T = V dO^T over 64-key stages up to
+//    the diagonal, then dQ^T += K^T dS^T.  Its prologue forms delta.
+//  * packed_bwd_dkdv: 128 keys of one key / value head, 32 a wave, one a lane; over 32-query stages from the diagonal on,
+//    for one query head of the group after the other, S = Q K^T and dP = dO V^T, then dV^T += dO^T P, dK^T += Q^T dS.
+//    With few key tiles the group's heads are split over several workgroups, whose fp32 parts packed_bwd_sum adds in order.
+// Stages that a wave does not see at all are skipped, those on the diagonal (or at a sequence's end) masked.
+// P and dS are rounded to the 16-bit type as operands, the gradients once at the end.
+#include "packed.h"
+
+namespace vmo {
+
+constexpr int kDqKeys = 64;      // keys of a dq stage
+constexpr int kKvQueries = 32;   // queries of a dk / dv stage
+
+template <int D> constexpr int packed_dq_lds() {
+  constexpr int ring = 2 * kDqKeys * D * 2 * 2;
+  constexpr int least = kPackedWaves * kEpiPatchBytes > 12 * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : 12 * kPackedMaxSeqs;
+  return ring > least ? ring : least;
+}
+// V's 128 rows in LDS at D = 128 (in registers they would spill)
+template <int D> constexpr bool packed_v_in_lds() { return D >= 128; }
+template <int D> constexpr int packed_kv_stage() { return kKvQueries * D * 2 * 2 + 512; }
+template <int D> constexpr int packed_kv_lds() {
+  constexpr int ring = 2 * packed_kv_stage<D>() + (packed_v_in_lds<D>() ? kPackedTile * D * 2 : 0);
+  constexpr int least = kPackedWaves * kEpiPatchBytes > 12 * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : 12 * kPackedMaxSeqs;
+  return ring > least ? ring : least;
+}
+
+template <class V8, int RB>
+__device__ __forceinline__ V8 packed_tr(const VMO_LDS char* block16, int trow, int tchunk, int tbyte, int a) {
+  const int c0 = trow * RB + (((4 * a + tchunk) ^ swz_rows<RB>(trow)) * 16 + tbyte);
+  return lds_read_tr8<V8>(block16 + c0, block16 + 8 * RB + (c0 ^ 32));
+}
+
+template <bool F16, int D>
+__global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(PackedParams p) {
+  using E = Elem<F16>;
+  using T = typename E::T;
+  using V8 = typename E::V8;
+  constexpr int RB = D * 2, K_BYTES = kDqKeys * RB, STAGE = 2 * K_BYTES, NA = D / 32, NDS = D / 16;
+  constexpr int PF = D <= 64 ? 0 : 2;   // operand reads in flight ahead of their product
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  VMO_LDS char* smem = (VMO_LDS char*)smem_raw;
+  const uint32_t smem_u32 = (uint32_t)(uintptr_t)smem;
+  auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
+
+  const int head = uni(packed_head((int)blockIdx.x % p.heads, p.heads));
+  const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, (VMO_LDS int*)smem);
+  if (w.tile < 0) {
+    packed_zero_rest<T, D>((T*)p.dq + head * p.dq_sh, p.dq_sn, p.q_off, p.n, p.tq, w.seq, w.spare);
+    return;
+  }
+  const PackedSeq sq = packed_seq(p, uni(w.seq));
+  const int nq = uni(sq.nq), nk = uni(sq.nk), qb = uni(sq.qb), kb = uni(sq.kb);
+  const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
+  const int q0 = uni(w.tile) * kPackedTile + wave * 32;
+  const bool live = q0 < nq;
+  const int past = nk - nq;
+  auto keys_of = [&](int row) __attribute__((always_inline)) { return p.causal ? min(max(past + row + 1, 0), nk) : nk; };
+  const int row = min(q0 + l32, nq - 1);
+  const int lim = keys_of(row);
+  const int lo = uni(keys_of(min(q0, nq - 1))), hi = uni(keys_of(min(q0 + 31, nq - 1)));
+  const int n_tiles = uni((keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 1, nq - 1)) + kDqKeys - 1) / kDqKeys);
+
+  // Q^T and dO^T as B operands (one query a lane); delta in fp32
+  V8 qf[NDS], dof[NDS];
+  float delta = 0.f;
+  const int64_t tok = qb + row;
+  {
+    const T* qp = (const T*)p.q + (int64_t)head * p.q_sh + tok * p.q_sn + hl * 8;
+    const T* dp = (const T*)p.dO + (int64_t)head * p.do_sh + tok * p.do_sn + hl * 8;
+    const T* op = (const T*)p.o + (int64_t)head * p.o_sh + tok * p.o_sn + hl * 8;
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) {
+      qf[ds] = *(const V8*)(qp + ds * 16);
+      asm volatile("" : "+v"(qf[ds]));
+    }
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) {
+      dof[ds] = *(const V8*)(dp + ds * 16);
+      asm volatile("" : "+v"(dof[ds]));
+      const V8 y = *(const V8*)(op + ds * 16);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf((float)dof[ds][e], (float)y[e], delta);
+    }
+  }
+  float alpha = -wave_sum32(delta);
+  float lse = p.lse[(int64_t)head * p.st_sh + tok];
+  asm volatile("" : "+v"(alpha), "+v"(lse));   // waited for here: a wait in the loop would also wait for the copies
+  if (live && hl == 0 && q0 + l32 < nq) p.neg_delta[(int64_t)head * p.tq + tok] = alpha;
+
+  const T* kbase = (const T*)p.k + (int64_t)(head / p.group) * p.k_sh + (int64_t)kb * p.k_sn;
+  const T* vbase = (const T*)p.v + (int64_t)(head / p.group) * p.v_sh + (int64_t)kb * p.v_sn;
+  const TileCopy<T, D, kPackedWaves> kcopy(kbase, p.k_sn, wave, lane), vcopy(vbase, p.v_sn, wave, lane);
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    const uint32_t st = smem_u32 + (uint32_t)((t & 1) * STAGE);
+    kcopy.issue(t * kDqKeys, nk, st);
+    vcopy.issue(t * kDqKeys, nk, st + K_BYTES);
+  };
+  f32x16 acc[NA];
+#pragma unroll
+  for (int a = 0; a < NA; ++a) acc[a] = f32x16{};
+  const float c = p.c;
+  const int sw = swz_rows<RB>(l32);
+  const int trow = 4 * hl + ((lane & 15) >> 2), tchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), tbyte = (lane & 1) * 8;
+
+  auto stage = [&](int t, auto masked_tag) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
+    const VMO_LDS char* Ks = smem + (t & 1) * STAGE;
+    const VMO_LDS char* Vs = Ks + K_BYTES;
+    f32x16 s[2] = {f32x16{}, f32x16{}}, dp[2] = {f32x16{}, f32x16{}};
+    prefetched_chain<4 * NDS, PF>(
+        [&](int i) __attribute__((always_inline)) {
+          const int kb2 = i / (2 * NDS), j = i % (2 * NDS);
+          return lds_read8<V8>((j < NDS ? Ks : Vs) + (32 * kb2 + l32) * RB + ((2 * (j % NDS) + hl) ^ sw) * 16);
+        },
+        [&](int i, const V8& x) __attribute__((always_inline)) {
+          const int kb2 = i / (2 * NDS), j = i % (2 * NDS);
+          if (j < NDS) s[kb2] = E::mfma(x, qf[j], s[kb2]);
+          else dp[kb2] = E::mfma(x, dof[j - NDS], dp[kb2]);
+        });
+    if constexpr (PF > 0) {
+      struct Chain {
+        static constexpr int reads(int) { return 1; }
+        static constexpr int mfmas(int) { return 1; }
+        static constexpr int ahead(int) { return 2; }
+        static constexpr int lead() { return 0; }
+      };
+      pin_chain<Chain, 4 * NDS>();
+    }
+    V8 G[2][2];
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float g = fast_exp2(fmaf(s[kb2][r], c, -lse)) * (dp[kb2][r] + alpha);
+        if (MASKED) g = t * kDqKeys + 32 * kb2 + 8 * (r >> 2) + 4 * hl + (r & 3) < lim ? g : 0.f;
+        G[kb2][r >> 3][r & 7] = to_elem<T>(g);
+      }
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int kb2 = 0; kb2 < 2; ++kb2) {
+        const int nvis = lim - t * kDqKeys - 32 * kb2;
+        masked_product<F16, RB>(acc, Ks + 32 * kb2 * RB, G[kb2], lane, [&](int key) { return key < nvis; });
+      }
+    } else {
+      prefetched_chain<4 * NA, PF>(
+          [&](int i) __attribute__((always_inline)) {
+            return packed_tr<V8, RB>(Ks + 16 * (i % 4) * RB, trow, tchunk, tbyte, i / 4);
+          },
+          [&](int i, const V8& x) __attribute__((always_inline)) {
+            acc[i / 4] = E::mfma(x, G[(i % 4) >> 1][i & 1], acc[i / 4]);
+          });
+    }
+  };
+  if (n_tiles > 0) {
+    issue(0);
+    const int n_full = live ? uni(min(lo / kDqKeys, n_tiles)) : 0;
+    auto top = [&](int t) __attribute__((always_inline)) {
+      tile_sync<0>();   // stage t has landed for every wave, and stage t - 1's slot is free
+      if (t + 1 < n_tiles) issue(t + 1);
+    };
+    int t = 0;
+    for (; t < n_full; ++t) {
+      top(t);
+      stage(t, std::false_type{});
+    }
+    for (; t < n_tiles; ++t) {
+      top(t);
+      if (live && t * kDqKeys < hi) stage(t, std::true_type{});
+    }
+  }
+  __syncthreads();
+  if (!live) return;
+  T* out = (T*)p.dq + (int64_t)head * p.dq_sh + (int64_t)(qb + q0) * p.dq_sn;
+  store_acc_rows<F16>((VMO_LDS float*)(smem + wave * kEpiPatchBytes), acc, NA, p.sm_scale, kGradStore, (char*)out, p.dq_sn * 2,
+                      min(32, nq - q0), lane);
+}
+
+template <bool F16, int D>
+__global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(PackedParams p) {
+  using E = Elem<F16>;
+  using T = typename E::T;
+  using V8 = typename E::V8;
+  constexpr int RB = D * 2, Q_BYTES = kKvQueries * RB, STAGE = packed_kv_stage<D>(), NA = D / 32, NDS = D / 16;
+  constexpr bool V_LDS = packed_v_in_lds<D>();
+  constexpr int PF = 2;
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  VMO_LDS char* smem = (VMO_LDS char*)smem_raw;
+  const uint32_t smem_u32 = (uint32_t)(uintptr_t)smem;
+  auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
+
+  const int shares = p.kv_heads * p.splits;   // workgroups of one key tile
+  const int hs = uni(packed_head((int)blockIdx.x % shares, shares));
+  const int kvh = hs / p.splits, split = hs % p.splits;
+  const PackedTile w = packed_locate<true>(p, (int)blockIdx.x / shares, (int)gridDim.x / shares, (VMO_LDS int*)smem);
+  if (w.tile < 0) {
+    if (p.splits == 1) {
+      packed_zero_rest<T, D>((T*)p.dk + kvh * p.dk_sh, p.dk_sn, p.k_off, p.n, p.tk, w.seq, w.spare);
+      packed_zero_rest<T, D>((T*)p.dv + kvh * p.dv_sh, p.dv_sn, p.k_off, p.n, p.tk, w.seq, w.spare);
+    }
+    return;
+  }
+  const PackedSeq sq = packed_seq(p, uni(w.seq));
+  const int nq = uni(sq.nq), nk = uni(sq.nk), qb = uni(sq.qb), kb = uni(sq.kb);
+  const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
+  const int tile0 = uni(w.tile) * kPackedTile, k0 = tile0 + wave * 32;
+  const bool live = k0 < nk;
+  const int key = min(k0 + l32, nk - 1);
+  // the first row that sees a key, counted from the wave's and the workgroup's first keys
+  const int past = nk - nq;
+  auto first_row = [&](int j) __attribute__((always_inline)) { return p.causal ? max(j - past, 0) : 0; };
+  const int from = first_row(key);
+  const int w_from = uni(first_row(min(k0, nk - 1))), w_whole = uni(first_row(min(k0 + 31, nk - 1)));
+  const int t0 = uni(first_row(tile0) / kKvQueries), t1 = uni((nq + kKvQueries - 1) / kKvQueries);
+  const int per = p.group / p.splits, h0 = kvh * p.group + split * per;
+  const int steps = t1 > t0 ? t1 - t0 : 0, n_it = uni(steps * per);
+
+  const T* kp0 = (const T*)p.k + (int64_t)kvh * p.k_sh + (int64_t)kb * p.k_sn;
+  const T* vp0 = (const T*)p.v + (int64_t)kvh * p.v_sh + (int64_t)kb * p.v_sn;
+  V8 kf[NDS], vf[V_LDS ? 1 : NDS];
+#pragma unroll
+  for (int ds = 0; ds < NDS; ++ds) {
+    kf[ds] = *(const V8*)(kp0 + (int64_t)key * p.k_sn + hl * 8 + ds * 16);
+    asm volatile("" : "+v"(kf[ds]));
+  }
+  const VMO_LDS char* vt_row = smem + 2 * STAGE + (wave * 32 + l32) * RB;
+  if constexpr (V_LDS) {   // the workgroup's 128 V rows, once (landed by the first tile_sync)
+    const TileCopy<T, D, kPackedWaves, D, kPackedTile> vrows(vp0, p.v_sn, wave, lane);
+    vrows.issue(tile0, nk, smem_u32 + 2 * STAGE);
+  } else {
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) {
+      vf[ds] = *(const V8*)(vp0 + (int64_t)key * p.v_sn + hl * 8 + ds * 16);
+      asm volatile("" : "+v"(vf[ds]));
+    }
+  }
+
+  TileCopy<T, D, kPackedWaves, D, kKvQueries> qcopy((const T*)p.q + (int64_t)h0 * p.q_sh + (int64_t)qb * p.q_sn, p.q_sn, wave, lane);
+  TileCopy<T, D, kPackedWaves, D, kKvQueries> docopy((const T*)p.dO + (int64_t)h0 * p.do_sh + (int64_t)qb * p.do_sn, p.do_sn, wave,
+                                                     lane);
+  const float* lse_h = p.lse + (int64_t)h0 * p.st_sh + qb;
+  const float* nd_h = p.neg_delta + (int64_t)h0 * p.tq + qb;
+  int t_next = t0;   // the stage that the next issue copies; past the last one comes the next head's first
+  auto issue = [&](int slot) __attribute__((always_inline)) {
+    const uint32_t st = smem_u32 + (uint32_t)(slot * STAGE);
+    const int row0 = t_next * kKvQueries;
+    qcopy.issue(row0, nq, st);
+    docopy.issue(row0, nq, st + Q_BYTES);
+    if (wave == 0) {   // lanes 0-31: lse, 32-63: -delta
+      const int qi = min(row0 + l32, nq - 1);
+      dma4_async(hl ? nd_h + qi : lse_h + qi, st + 2 * Q_BYTES);
+    }
+    if (++t_next == t1) {
+      t_next = t0;
+      qcopy.ubase = uniform64(qcopy.ubase + (uint64_t)p.q_sh * 2);
+      docopy.ubase = uniform64(docopy.ubase + (uint64_t)p.do_sh * 2);
+      lse_h += p.st_sh;
+      nd_h += p.tq;
+    }
+  };
+
+  f32x16 dk[NA], dv[NA];
+#pragma unroll
+  for (int a = 0; a < NA; ++a) dk[a] = dv[a] = f32x16{};
+  const float c = p.c;
+  const int sw = swz_rows<RB>(l32);
+  const int trow = 4 * hl + ((lane & 15) >> 2), tchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), tbyte = (lane & 1) * 8;
+
+  auto stage = [&](int slot, int row0, auto masked_tag) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
+    const VMO_LDS char* Qs = smem + slot * STAGE;
+    const VMO_LDS char* dOs = Qs + Q_BYTES;
+    const VMO_LDS float* sts = (const VMO_LDS float*)(dOs + Q_BYTES);
+    f32x16 s = f32x16{}, dp;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {   // dP starts from -delta
+      const f32x4 av = *(const VMO_LDS f32x4*)(sts + 32 + 8 * g + 4 * hl);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * g + e] = av[e];
+    }
+    struct Ops { V8 a, b; };
+    prefetched_chain<2 * NDS, PF>(
+        [&](int i) __attribute__((always_inline)) {
+          Ops o;
+          const int off = ((2 * (i % NDS) + hl) ^ sw) * 16;
+          o.a = lds_read8<V8>((i < NDS ? Qs : dOs) + l32 * RB + off);
+          o.b = i < NDS ? kf[i] : V_LDS ? lds_read8<V8>(vt_row + off) : vf[V_LDS ? 0 : i - NDS];
+          return o;
+        },
+        [&](int i, const Ops& o) __attribute__((always_inline)) {
+          if (i < NDS) s = E::mfma(o.a, o.b, s);
+          else dp = E::mfma(o.a, o.b, dp);
+        });
+    struct Chain {
+      static constexpr int reads(int i) { return i < NDS ? 1 : 1 + (V_LDS ? 1 : 0); }
+      static constexpr int mfmas(int) { return 1; }
+      static constexpr int ahead(int) { return 2; }
+      static constexpr int lead() { return 4; }
+    };
+    pin_chain<Chain, 2 * NDS>();
+    auto sees = [&](int r) __attribute__((always_inline)) { return row0 + r >= from && row0 + r < nq; };
+    V8 P[2], G[2];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 lv = *(const VMO_LDS f32x4*)(sts + 8 * g + 4 * hl);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * g + e;
+        float pv = fast_exp2(fmaf(s[r], c, -lv[e]));
+        float gv = pv * dp[r];
+        if (MASKED) {
+          const bool ok = sees(8 * g + 4 * hl + e);
+          pv = ok ? pv : 0.f;
+          gv = ok ? gv : 0.f;
+        }
+        P[r >> 3][r & 7] = to_elem<T>(pv);
+        G[r >> 3][r & 7] = to_elem<T>(gv);
+      }
+    }
+    if constexpr (MASKED) {
+      masked_product<F16, RB>(dv, dOs, P, lane, sees);
+      masked_product<F16, RB>(dk, Qs, G, lane, sees);
+    } else {
+      prefetched_chain<4 * NA, PF>(
+          [&](int i) __attribute__((always_inline)) {
+            return packed_tr<V8, RB>((i < 2 * NA ? dOs : Qs) + 16 * (i % 2) * RB, trow, tchunk, tbyte, (i / 2) % NA);
+          },
+          [&](int i, const V8& x) __attribute__((always_inline)) {
+            if (i < 2 * NA) dv[i / 2] = E::mfma(x, P[i % 2], dv[i / 2]);
+            else dk[i / 2 - NA] = E::mfma(x, G[i % 2], dk[i / 2 - NA]);
+          });
+    }
+  };
+  if (n_it > 0) {
+    issue(0);
+    // a head's stages: those before the wave's keys are seen whole, those that its 32 keys see whole, the partial last one
+    // (three loops: with both kinds in one body the compiler spills the accumulators)
+    const int a0 = min(max((w_whole + kKvQueries - 1) / kKvQueries, t0), t1), a1 = live ? max(nq / kKvQueries, a0) : a0;
+    int it = 0;
+    auto top = [&]() __attribute__((always_inline)) {
+      tile_sync<0>();   // this stage has landed for every wave, and the other slot is free
+      if (it + 1 < n_it) issue((it + 1) & 1);
+    };
+    auto masked = [&](int t) __attribute__((always_inline)) {
+      top();
+      if (live && (t + 1) * kKvQueries > w_from) stage(it & 1, t * kKvQueries, std::true_type{});
+      ++it;
+    };
+    for (int h = 0; h < per; ++h) {
+      int t = t0;
+      const int upto = live ? a0 : t1;
+      for (; t < upto; ++t) masked(t);
+      for (; t < a1; ++t) {
+        top();
+        stage(it & 1, t * kKvQueries, std::false_type{});
+        ++it;
+      }
+      for (; t < t1; ++t) masked(t);
+    }
+  } else {
+    tile_sync<0>();   // V's copies have landed before the patches take their place
+  }
+  __syncthreads();
+  if (!live) return;
+  VMO_LDS float* patch = (VMO_LDS float*)(smem + wave * kEpiPatchBytes);
+  const int nrows = min(32, nk - k0);
+  if (p.splits > 1) {
+    const int64_t r = ((int64_t)(split * p.kv_heads + kvh) * p.tk + kb + k0) * D;
+    store_acc_rows<F16>(patch, dk, NA, p.sm_scale, kGradStoreF32, (char*)(p.dk_part + r), D * 4, nrows, lane);
+    store_acc_rows<F16>(patch, dv, NA, 1.0f, kGradStoreF32, (char*)(p.dv_part + r), D * 4, nrows, lane);
+  } else {
+    store_acc_rows<F16>(patch, dk, NA, p.sm_scale, kGradStore,
+                        (char*)((T*)p.dk + (int64_t)kvh * p.dk_sh + (int64_t)(kb + k0) * p.dk_sn), p.dk_sn * 2, nrows, lane);
+    store_acc_rows<F16>(patch, dv, NA, 1.0f, kGradStore,
+                        (char*)((T*)p.dv + (int64_t)kvh * p.dv_sh + (int64_t)(kb + k0) * p.dv_sn), p.dv_sn * 2, nrows, lane);
+  }
+}
+
+// dk and dv from their parts, in the parts' order; rows outside every sequence (they have no parts) are zeros.
+template <bool F16, int D>
+__global__ __launch_bounds__(256) void packed_bwd_sum_kernel(PackedParams p) {
+  using T = typename Elem<F16>::T;
+  using V4 = typename Elem<F16>::V4;
+  constexpr int TPR = D / 4;
+  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t rows = (int64_t)p.kv_heads * p.tk, r = gid / TPR;
+  const int c4 = (int)(gid % TPR) * 4;
+  if (r >= rows) return;
+  const int kvh = (int)(r / p.tk), tok = (int)(r % p.tk);
+  f32x4 a = f32x4{}, b = f32x4{};
+  if (tok >= min(max(p.k_off[0], 0), p.tk) && tok < min(max(p.k_off[p.n], 0), p.tk))
+    for (int s = 0; s < p.splits; ++s) {
+      const int64_t at = (s * rows + r) * D + c4;
+      a += *(const f32x4*)(p.dk_part + at);
+      b += *(const f32x4*)(p.dv_part + at);
+    }
+  V4 x, y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] = to_elem<T>(a[e]);
+    y[e] = to_elem<T>(b[e]);
+  }
+  *(V4*)((T*)p.dk + (int64_t)kvh * p.dk_sh + (int64_t)tok * p.dk_sn + c4) = x;
+  *(V4*)((T*)p.dv + (int64_t)kvh * p.dv_sh + (int64_t)tok * p.dv_sn + c4) = y;
+}
+
+// Workgroups that share a key tile: as many as divide the group and bring the launch to two rounds of the chip's slots
+// (256 CUs, two workgroups each).
+int packed_bwd_splits(int64_t tk, int n, int kv_heads, int group) {
+  const int64_t tiles = ((tk + kPackedTile - 1) / kPackedTile) * kv_heads;
+  int splits = 1;
+  while (splits < group && tiles * splits < 1024) {
+    int next = splits + 1;
+    while (group % next) ++next;
+    splits = next;
+  }
+  return splits;
+}
+
+template <bool F16, int D>
+static int launch_packed_bwd(const PackedParams& p, hipStream_t s) {
+  constexpr int LDS_Q = packed_dq_lds<D>(), LDS_KV = packed_kv_lds<D>();
+  static_assert(LDS_Q <= 65536 && LDS_KV <= 80 * 1024, "two workgroups a CU");
+  if (p.tq > 0) {
+    const int64_t grid = ((int64_t)(p.tq + kPackedTile - 1) / kPackedTile + p.n) * p.heads;
+    hipLaunchKernelGGL((packed_bwd_dq_kernel<F16, D>), dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_Q, s, p);
+    const int rc = launch_status("packed_bwd_dq");
+    if (rc != VMO_OK) return rc;
+  }
+  if (p.tk == 0) return VMO_OK;
+  auto kern = packed_bwd_dkdv_kernel<F16, D>;
+  if (LDS_KV > 65536 &&
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_KV) != hipSuccess)
+    return set_error(VMO_ERR_LAUNCH, "packed_bwd: cannot raise the LDS limit to %d bytes", LDS_KV);
+  const int64_t grid = ((int64_t)(p.tk + kPackedTile - 1) / kPackedTile + p.n) * p.kv_heads * p.splits;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_KV, s, p);
+  const int rc = launch_status("packed_bwd_dkdv");
+  if (rc != VMO_OK || p.splits == 1) return rc;
+  const int64_t threads = (int64_t)p.kv_heads * p.tk * (D / 4);
+  hipLaunchKernelGGL((packed_bwd_sum_kernel<F16, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
+  return launch_status("packed_bwd_sum");
+}
+
+int packed_bwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s) {
+  if (d == 64) return f16 ? launch_packed_bwd<true, 64>(p, s) : launch_packed_bwd<false, 64>(p, s);
+  return f16 ? launch_packed_bwd<true, 128>(p, s) : launch_packed_bwd<false, 128>(p, s);
+}
+
+}  // namespace vmo
