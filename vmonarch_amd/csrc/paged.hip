@@ -269,10 +269,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   const int id = p.table[(int64_t)b * p.t_sb + (at >> p.page_log)];
   if (id < 0 || id >= p.pages) return;
   const int64_t place = at & ((1 << p.page_log) - 1);
-  *(uint4*)((char*)p.kp + (id * p.k_sp + h * p.kp_sh + place * p.kp_sn) * 2 + ch * 16) =
-      *(const uint4*)((const char*)p.k + (h * p.k_sh + row * p.k_sn) * 2 + ch * 16);
-  *(uint4*)((char*)p.vp + (id * p.v_sp + h * p.vp_sh + place * p.vp_sn) * 2 + ch * 16) =
-      *(const uint4*)((const char*)p.v + (h * p.v_sh + row * p.v_sn) * 2 + ch * 16);
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 x = *(const u32x4*)((const char*)p.k + (h * p.k_sh + row * p.k_sn) * 2 + ch * 16);
+  const u32x4 y = *(const u32x4*)((const char*)p.v + (h * p.v_sh + row * p.v_sn) * 2 + ch * 16);
+  *(u32x4*)((char*)p.kp + (id * p.k_sp + h * p.kp_sh + place * p.kp_sn) * 2 + ch * 16) = x;
+  *(u32x4*)((char*)p.vp + (id * p.v_sp + h * p.vp_sh + place * p.vp_sn) * 2 + ch * 16) = y;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -283,22 +284,18 @@ struct CopyParams {
   int pairs, pieces;
   int32_t src[kCopyPairs], dst[kCopyPairs];
 };
-constexpr int kCopyPiece = 256 * 16 * 4;   // bytes a workgroup moves
+constexpr int kCopyPiece = 256 * 16;   // bytes a workgroup moves
 
-// Pages src[i] to dst[i] of every layer, K and V: 16 KB a workgroup, four loads in flight a lane.
+// Pages src[i] to dst[i] of every layer, K and V.  Bound by memory, the small copies by the launch: one 16-byte piece a
+// lane (12 layers x 256 pages of 16 KB: 24.0 us against 26.1 with four a lane, whose fewer workgroups also start slower: 32
+// pages 3.4 against 4.4 us), stored past the caches (3.4 against 3.9 us).
 __global__ __launch_bounds__(256) void paged_copy_kernel(CopyParams p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));   // (HIP's own uint4 went through registers one at a time)
   const int piece = (int)blockIdx.x % p.pieces, pair = (int)blockIdx.x / p.pieces, layer = (int)blockIdx.y;
   char* base = (blockIdx.z ? p.v : p.k) + layer * p.layer_bytes;
-  const char* from = base + p.src[pair] * p.page_bytes;
-  char* to = base + p.dst[pair] * p.page_bytes;
   const int64_t at = (int64_t)piece * kCopyPiece + threadIdx.x * 16;
-  uint4 x[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (at + i * 4096 < p.page_bytes) x[i] = *(const uint4*)(from + at + i * 4096);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (at + i * 4096 < p.page_bytes) *(uint4*)(to + at + i * 4096) = x[i];
+  if (at < p.page_bytes)
+    __builtin_nontemporal_store(*(const u32x4*)(base + p.src[pair] * p.page_bytes + at), (u32x4*)(base + p.dst[pair] * p.page_bytes + at));
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
