@@ -5,14 +5,12 @@
 // beyond the table, is not followed: attention gives NaN for that sequence, appending leaves the row out.
 #include <stdlib.h>
 
-#include "fea_fwd.h"
+#include "packed.h"
 
 namespace vmo {
 
-constexpr int kPagedWaves = 4;
-constexpr int kPagedTile = 32;        // keys of a wave's tile
-constexpr int kPagedMaxChunk = 2048;  // keys of a workgroup (their page numbers wait in LDS)
-constexpr float kPagedNoMax = -3.0e38f;
+constexpr int kPagedTile = 32;   // keys of a tile, one step of a wave
+constexpr float kPagedSumMost = 32768.f, kPagedNoMax = -3.0e38f;   // as in the forward of whole prompts
 
 struct PagedParams {
   const void *q, *k, *v;
@@ -21,216 +19,354 @@ struct PagedParams {
   const int32_t *table, *lengths;
   int64_t t_sb;
   int batch, heads, kv_heads, group, pages, page_log, width;   // width: page numbers a sequence has in the table
-  int chunk, chunks;                                           // keys a workgroup takes; workgroups a (sequence, head)
-  float *part_o, *part_ml;                                     // (batch, heads, chunks, D), (.., 2): sums, then m and l
+  int blocks, per;           // a sequence's rows: kv_heads x blocks of `per` (at most 32) query heads
+  int waves, q_rows;         // waves launched; query rows that an LDS slot holds (per, in whole copies)
+  float *part_o, *part_ml;   // (waves + batch kv_heads blocks) parts of (per, D), and of (per, 2): sums, then m and l
   float c;
 };
 
-// A sequence's length as the kernels take it: none below 0; `bad` beyond the table.
-__device__ __forceinline__ int paged_length(const PagedParams& p, int b, bool& bad) {
-  const int len = max(p.lengths[b], 0);
-  bad = len > ((int64_t)p.width << p.page_log);
-  return len;
+// A sequence's tiles.  One without tokens, or whose length is beyond the table (bad), has one that sees nothing: somebody
+// writes its rows.
+struct PagedSeq { int len, tiles; bool bad; };
+__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int len) {
+  PagedSeq s;
+  s.bad = len > ((int64_t)p.width << p.page_log);
+  s.len = s.bad ? 0 : max(len, 0);
+  s.tiles = max((s.len + kPagedTile - 1) / kPagedTile, 1);
+  return s;
 }
+// Tiles of all rows stand in one order (sequence, row of it, tile); wave w of W takes those from w total / W up to
+// (w + 1) total / W, so tile T belongs to wave ((T + 1) W - 1) / total.  A row that several waves hold has a part from each,
+// in place (wave + row): along the order one of the two grows with every part, so places are its own.
+__device__ __forceinline__ int64_t paged_owner(int64_t tile, int64_t waves, int64_t total) { return ((tile + 1) * waves - 1) / total; }
 
 // ------------------------------------------------------------------------------------------------
-// One workgroup: `chunk` keys of one (sequence, key / value head), all query heads of its group as the columns of the
-// 32-wide products (S^T = K Q^T, O^T += V^T P^T as the forward of whole prompts has them).  A wave takes every fourth tile
-// of 32 keys through its own two LDS slots (its copies need no barrier: nobody else reads them), with its own running
-// maximum and sum; the four waves are joined in LDS, the workgroups of a sequence by paged_join.
-// Bound by the bytes of the cache: 2 D 2 bytes a key and head.
+// A wave is a workgroup of its own and walks its share of the tiles, over the ends of sequences: 32 keys of one key / value
+// head against the query heads of its group, the columns of the 32-wide products (S^T = K Q^T, O^T += V^T P^T, a lane one
+// query head, as in the forward of whole prompts).  K and V tiles have two LDS slots each; K of tile i + 2 is fetched when
+// S of tile i is formed, V of it when P V is, so three quarters of the wave's LDS is always under way, and no barrier is
+// met.  Page numbers and lengths come through the scalar unit, whose waits leave the copies alone; a copy instruction lies
+// within one page (pages hold 8 tokens at least), so its address is scalar too.
+// Bound by the bytes of the cache, 2 D 2 a key and head, and by how many of them are in flight.
 template <bool F16, int D>
-__global__ __launch_bounds__(64 * kPagedWaves) void paged_attention_kernel(PagedParams p) {
+__global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams p) {
   using E = Elem<F16>;
   using T = typename E::T;
   using V8 = typename E::V8;
-  constexpr int RB = D * 2, K_BYTES = kPagedTile * RB, SLOT = 2 * K_BYTES, NA = D / 32, NDS = D / 16;
-  constexpr int CH = D / 8, RPI = 64 / CH, NI = kPagedTile / RPI;   // copies of a K (or V) tile by one wave
+  typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+  constexpr int RB = D * 2, UNIT = kPagedTile * RB, NA = D / 32, NDS = D / 16;
+  constexpr int CH = D / 8, RPI = 64 / CH, NI = kPagedTile / RPI;   // copies of a K (or V) tile
+  constexpr int NV = 16 / RPI;                                      // lane offsets: the swizzle's period is 16 rows
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
   VMO_LDS char* smem = (VMO_LDS char*)smem_raw;
-  VMO_LDS int* ids = (VMO_LDS int*)(smem + kPagedWaves * 2 * SLOT);   // the chunk's page numbers, then a flag
+  const uint32_t lds = (uint32_t)(uintptr_t)smem;
   auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
+  const int lane = threadIdx.x, hl = lane >> 5, l32 = lane & 31;
+  const scalar_ints lengths = (scalar_ints)(uintptr_t)p.lengths, table = (scalar_ints)(uintptr_t)p.table;
+  const int X = p.kv_heads * p.blocks;   // rows of a sequence
 
-  const int chunk = (int)blockIdx.x % p.chunks, bh = (int)blockIdx.x / p.chunks;
-  const int kvh = bh % p.kv_heads, b = bh / p.kv_heads;
-  const int h0 = kvh * p.group + (int)blockIdx.y * 32, nh = min(32, p.group - (int)blockIdx.y * 32);
-  const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
-  bool bad;
-  const int len = uni(paged_length(p, b, bad));
-  const int beg = chunk * p.chunk;
-  if (beg >= len && !(chunk == 0)) return;
-  const int end = min(len, beg + p.chunk);
-  int n_keys = bad ? 0 : max(end - beg, 0);
-
-  // page numbers of the chunk, checked
-  const int page0 = beg >> p.page_log, n_pages = n_keys > 0 ? ((beg + n_keys - 1) >> p.page_log) - page0 + 1 : 0;
-  bool wrong = bad;
-  for (int i = tid; i < n_pages; i += 64 * kPagedWaves) {
-    const int id = p.table[(int64_t)b * p.t_sb + page0 + i];
-    wrong |= id < 0 || id >= p.pages;
-    ids[i] = min(max(id, 0), p.pages - 1);
-  }
-  const int any_wrong = __syncthreads_or(wrong);
-
-  V8 qf[NDS];
-  {
-    const T* qp = (const T*)p.q + (int64_t)b * p.q_sb + (int64_t)(h0 + min(l32, nh - 1)) * p.q_sh + hl * 8;
+  // this wave's tiles
+  int64_t sum = 0;
+  for (int b = lane; b < p.batch; b += 64) sum += paged_seq(p, p.lengths[b]).tiles;
 #pragma unroll
-    for (int ds = 0; ds < NDS; ++ds) {
-      qf[ds] = *(const V8*)(qp + ds * 16);
-      asm volatile("" : "+v"(qf[ds]));
+  for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
+  const int64_t total = uniform64((uint64_t)sum) * X;
+  const int64_t W = p.waves < total ? p.waves : total, w = blockIdx.x;
+  if (w >= W) return;
+  const int64_t first = w * total / W;
+  const int n = (int)((w + 1) * total / W - first);
+  int b = 0;
+  int64_t before = 0;   // tiles of the sequences before b, of one row
+  for (int s0 = 0;; s0 += 64) {
+    const int tiles = s0 + lane < p.batch ? paged_seq(p, p.lengths[s0 + lane]).tiles : 0;
+    const int upto = wave_scan_i32(tiles), all = __builtin_amdgcn_readlane(upto, 63);
+    if ((before + all) * X > first) {
+      const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64((before + upto) * X > first));
+      b = s0 + who;
+      before += __builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(tiles, who);
+      break;
     }
+    before += all;
   }
-  const int n_tiles = (n_keys + kPagedTile - 1) / kPagedTile;
-  const int mine = n_tiles > wave ? (n_tiles - wave + kPagedWaves - 1) / kPagedWaves : 0;
-  const uint32_t ring = (uint32_t)(uintptr_t)smem + wave * 2 * SLOT;
-  const char* kp = (const char*)p.k + (int64_t)kvh * p.k_sh * 2;
-  const char* vp = (const char*)p.v + (int64_t)kvh * p.v_sh * 2;
-  auto issue = [&](int i) __attribute__((always_inline)) {
-    const uint32_t st = ring + (i & 1) * SLOT;
-    const int key0 = beg + (wave + i * kPagedWaves) * kPagedTile;
+  struct Cursor { int b, x, tile; PagedSeq s; };   // row x of sequence b, its tile
+  Cursor at;
+  at.b = uni(b);
+  at.s = paged_seq(p, lengths[at.b]);
+  const int64_t rest = first - before * X;
+  at.x = uni((int)(rest / at.s.tiles));
+  at.tile = uni((int)(rest % at.s.tiles));
+  auto advance = [&](Cursor& c) __attribute__((always_inline)) {
+    if (++c.tile < c.s.tiles) return;
+    c.tile = 0;
+    if (++c.x < X) return;
+    c.x = 0;
+    c.b = min(c.b + 1, p.batch - 1);
+    c.s = paged_seq(p, lengths[c.b]);
+  };
+
+  // lane offsets of the copies (rows r0 + lane / CH of a tile, chunks swizzled by the row)
+  uint32_t koff[NV], voff[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int r = j * RPI + lane / CH;
+    const uint32_t chunk = ((lane % CH) ^ swz_rows<RB>(r)) * 16;
+    koff[j] = (uint32_t)((lane / CH) * p.k_sn * 2) + chunk;
+    voff[j] = (uint32_t)((lane / CH) * p.v_sn * 2) + chunk;
+  }
+  // The tile under `next`: its page numbers, then K (with the row's queries where it begins one, or the wave does), then V.
+  // ids[j]: the page of rows 8 j .. 8 j + 7.  A number outside the cache is not followed: page 0 instead, and the row is
+  // marked (bit i % 4 of `wrong`).
+  Cursor next = at;
+  int ids[4];
+  uint32_t wrong = 0;
+  const int place_mask = (1 << p.page_log) - 1;
+  auto pages_of_tile = [&](int i) __attribute__((always_inline)) {
+    const int64_t row = next.b * p.t_sb;
+    const int key0 = next.tile * kPagedTile, last = (next.s.len - 1) >> p.page_log;
+    bool bad = next.s.bad;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int page = min((key0 + 8 * j) >> p.page_log, last);
+      int id = 0;
+      if (next.s.len > 0) id = table[row + page];
+      const bool out = id < 0 || id >= p.pages;
+      bad |= out;
+      ids[j] = out ? 0 : id;
+    }
+    wrong = (wrong & ~(1u << (i & 3))) | (bad ? 1u << (i & 3) : 0u);
+  };
+  auto copy_tile = [&](const void* base, int64_t sp, int64_t sh, int64_t sn, const uint32_t (&off)[NV], uint32_t dst)
+      __attribute__((always_inline)) {
+    const uint64_t head = (uint64_t)(uintptr_t)base + (uint64_t)((next.x / p.blocks) * sh * 2);
+    const int key0 = next.tile * kPagedTile;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      const int r = j * RPI + lane / CH;
-      const int tok = min(key0 + r, end - 1);   // (keys past the end repeat the last one: masked)
-      const int64_t id = ids[(tok >> p.page_log) - page0], at = tok & ((1 << p.page_log) - 1);
-      const int byte = ((lane % CH) ^ swz_rows<RB>(r)) * 16;
-      dma16_async(kp + (id * p.k_sp + at * p.k_sn) * 2 + byte, st + j * 1024);
-      dma16_async(vp + (id * p.v_sp + at * p.v_sn) * 2 + byte, st + K_BYTES + j * 1024);
+      const int r = j * RPI;
+      dma16_async_s(head + (uint64_t)(ids[r / 8] * sp + ((key0 + r) & place_mask) * sn) * 2, off[j % NV], dst + j * 1024);
     }
   };
+  const uint32_t q_slots = lds + 4 * UNIT;
+  const int slot_bytes = p.q_rows * RB;
+  auto issue_k = [&](int i) __attribute__((always_inline)) {
+    pages_of_tile(i);
+    if (next.tile == 0 || i == 0) {
+      const int h0 = (next.x / p.blocks) * p.group + (next.x % p.blocks) * p.per, most = min(p.per, p.group - (next.x % p.blocks) * p.per) - 1;
+      for (int r = 0; r < p.q_rows; r += RPI)
+        dma16_async((const T*)p.q + next.b * p.q_sb + (h0 + min(r + lane / CH, most)) * p.q_sh + (lane % CH) * 8,
+                    q_slots + (i & 3) * slot_bytes + r * RB);
+    }
+    copy_tile(p.k, p.k_sp, p.k_sh, p.k_sn, koff, lds + (i & 1) * 2 * UNIT);
+  };
+  auto issue_v = [&](int i) __attribute__((always_inline)) {
+    copy_tile(p.v, p.v_sp, p.v_sh, p.v_sn, voff, lds + (i & 1) * 2 * UNIT + UNIT);
+    if (i + 1 < n) advance(next);
+  };
+  // waits until all but the newest `units` K or V tiles have landed
+  auto landed = [&](auto units) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(decltype(units)::value * NI) : "memory");
+  };
+  auto reads_done = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); };
+
   const float c = p.c;
+  V8 qf[NDS];
   float m_run = kPagedNoMax, l_run = 0.f;
   f32x16 acc[NA];
 #pragma unroll
   for (int a = 0; a < NA; ++a) acc[a] = f32x16{};
   const int sw = swz_rows<RB>(l32);
   const int trow = 4 * hl + ((lane & 15) >> 2), tchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), tbyte = (lane & 1) * 8;
+  bool begun = at.tile == 0, row_wrong = false;   // whether the wave has the row from its first tile
 
-  if (mine > 0) issue(0);
-  for (int i = 0; i < mine; ++i) {
-    if (i + 1 < mine) {
-      issue(i + 1);
-      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * NI) : "memory");   // tile i has landed, i + 1 is under way
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  issue_k(0);
+  issue_v(0);
+  if (n > 1) {
+    issue_k(1);
+    issue_v(1);
+  }
+  for (int i = 0; i < n; ++i) {
+    const VMO_LDS char* Ks = smem + (i & 1) * 2 * UNIT;
+    if (i + 1 < n) landed(std::integral_constant<int, 3>{});
+    else landed(std::integral_constant<int, 1>{});
+    const int nh = min(p.per, p.group - (at.x % p.blocks) * p.per);
+    if (at.tile == 0 || i == 0) {
+      const VMO_LDS char* qs = smem + 4 * UNIT + (i & 3) * slot_bytes + min(l32, nh - 1) * RB + hl * 16;
+#pragma unroll
+      for (int ds = 0; ds < NDS; ++ds) qf[ds] = lds_read8<V8>(qs + ds * 32);
     }
-    const VMO_LDS char* Ks = smem + wave * 2 * SLOT + (i & 1) * SLOT;
+    row_wrong |= (wrong >> (i & 3)) & 1;
     f32x16 s = f32x16{};
 #pragma unroll
-    for (int ds = 0; ds < NDS; ++ds)
-      s = E::mfma(lds_read8<V8>(Ks + l32 * RB + ((2 * ds + hl) ^ sw) * 16), qf[ds], s);
-    const int nvis = n_keys - (wave + i * kPagedWaves) * kPagedTile;
-    float mx = kPagedNoMax;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = 8 * (r >> 2) + 4 * hl + (r & 3) < nvis ? s[r] * c : -INFINITY;
-      mx = fmaxf(mx, s[r]);
-    }
-    const float m_new = fmaxf(m_run, wave_max32(mx)), f = fast_exp2(m_run - m_new);
-    m_run = m_new;
+    for (int ds = 0; ds < NDS; ++ds) s = E::mfma(lds_read8<V8>(Ks + l32 * RB + ((2 * ds + hl) ^ sw) * 16), qf[ds], s);
+    reads_done();
+    if (i + 2 < n) issue_k(i + 2);
+
+    const int nvis = at.s.len - at.tile * kPagedTile;   // keys of the tile that there are
     V8 P[2];
-    float ls = 0.f;
+    auto weights = [&]() __attribute__((always_inline)) {
+      float ls = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float x = fast_exp2(s[r] - m_run);
-      ls += x;
-      P[r >> 3][r & 7] = to_elem<T>(x);
+      for (int r = 0; r < 16; ++r) {
+        float x = fmaf(s[r], c, -m_run);
+        x = 8 * (r >> 2) + 4 * hl + (r & 3) < nvis ? x : kMaskLogit;
+        const float y = fast_exp2(x);
+        ls += y;
+        P[r >> 3][r & 7] = to_elem<T>(y);
+      }
+      return ls;
+    };
+    float ls = weights();
+    const bool over = !(ls <= kPagedSumMost);
+    if (__builtin_amdgcn_ballot_w64(over) != 0) {   // m moves to the row's maximum so far (see the forward of whole prompts)
+      const auto either = __builtin_amdgcn_permlane32_swap(over, over, false, false);
+      float mx = kPagedNoMax;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, 8 * (r >> 2) + 4 * hl + (r & 3) < nvis ? s[r] * c : kPagedNoMax);
+      const float m_new = either[0] | either[1] ? fmaxf(m_run, wave_max32(mx)) : m_run, f = fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_run *= f;
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[a][r] *= f;
+      ls = weights();
     }
-    l_run = fmaf(l_run, f, ls);
+    l_run += ls;
+
+    if (i + 2 < n) landed(std::integral_constant<int, 3>{});
+    else if (i + 1 < n) landed(std::integral_constant<int, 2>{});
+    else landed(std::integral_constant<int, 0>{});
+    if (nvis < kPagedTile) {   // places without a token hold anything: 0 times that need not be 0
+      const int gone = max(nvis, 0);
+      for (int j = lane; j < (kPagedTile - gone) * CH; j += 64)
+        *(VMO_LDS f32x4*)(smem + (i & 1) * 2 * UNIT + UNIT + gone * RB + j * 16) = f32x4{};
+      reads_done();
+    }
 #pragma unroll
     for (int a = 0; a < NA; ++a) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[a][r] *= f;
       const int c0 = trow * RB + (((4 * a + tchunk) ^ swz_rows<RB>(trow)) * 16 + tbyte);
 #pragma unroll
       for (int h2 = 0; h2 < 2; ++h2) {
-        const VMO_LDS char* rp = Ks + K_BYTES + 16 * h2 * RB;
+        const VMO_LDS char* rp = Ks + UNIT + 16 * h2 * RB;
         acc[a] = E::mfma(lds_read_tr8<V8>(rp + c0, rp + 8 * RB + (c0 ^ 32)), P[h2], acc[a]);
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");   // the slot's reads are done before it is filled again
-  }
-  // join the four waves: m and l of each (column, wave), then the sums scaled to the common m, added in the waves' order
-  __syncthreads();
-  VMO_LDS float* ml = (VMO_LDS float*)smem;                  // [wave][32][2]
-  VMO_LDS float* sums = (VMO_LDS float*)(smem + 1024);       // [wave][32][D + 4]
-  constexpr int SR = D + 4;
-  l_run = wave_sum32(l_run);
-  if (hl == 0) {
-    ml[(wave * 32 + l32) * 2] = m_run;
-    ml[(wave * 32 + l32) * 2 + 1] = l_run;
-  }
+    reads_done();
+    if (i + 2 < n) issue_v(i + 2);
+
+    const bool ends = at.tile + 1 == at.s.tiles;
+    if (ends || i + 1 == n) {   // the row is done here: whole, or this wave's part of it
+      float l = wave_sum32(l_run);
+      if (row_wrong) l = __uint_as_float(0x7fc00000u);   // NaN
+      const bool mine = l32 < nh;
+      if (ends && begun) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        T* out = (T*)p.o + at.b * p.o_sb + ((int64_t)(at.x / p.blocks) * p.group + (at.x % p.blocks) * p.per + l32) * p.o_sh;
 #pragma unroll
-  for (int a = 0; a < NA; ++a)
+        for (int a = 0; a < NA; ++a)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      f32x4 x;
+          for (int g = 0; g < 4; ++g) {
+            typename E::V4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = acc[a][4 * g + e];
-      if (l32 < nh) *(VMO_LDS f32x4*)(sums + (wave * 32 + l32) * SR + 32 * a + 8 * g + 4 * hl) = x;
-    }
-  __syncthreads();
-  const bool whole = p.chunks == 1;
-  for (int i = tid; i < nh * (D / 4); i += 64 * kPagedWaves) {
-    const int h = i / (D / 4), d4 = (i % (D / 4)) * 4;
-    float m = kPagedNoMax, l = 0.f;
+            for (int e = 0; e < 4; ++e) y[e] = to_elem<T>(acc[a][4 * g + e] * inv);
+            if (mine) *(typename E::V4*)(out + 32 * a + 8 * g + 4 * hl) = y;
+          }
+      } else {
+        const int64_t part = (w + (int64_t)at.b * X + at.x) * p.per + l32;
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) m = fmaxf(m, ml[(w * 32 + h) * 2]);
-    f32x4 x = f32x4{};
+        for (int a = 0; a < NA; ++a)
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) {
-      const float f = fast_exp2(ml[(w * 32 + h) * 2] - m);
-      l = fmaf(ml[(w * 32 + h) * 2 + 1], f, l);
-      const f32x4 y = *(const VMO_LDS f32x4*)(sums + (w * 32 + h) * SR + d4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = fmaf(y[e], f, x[e]);
-    }
-    if (any_wrong) l = __uint_as_float(0x7fc00000u);   // NaN: a page number or length that leads outside
-    if (whole) {
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      typename E::V4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = to_elem<T>(x[e] * inv);
-      *(typename E::V4*)((T*)p.o + (int64_t)b * p.o_sb + (int64_t)(h0 + h) * p.o_sh + d4) = y;
-    } else {
-      const int64_t at = ((int64_t)b * p.heads + h0 + h) * p.chunks + chunk;
-      *(f32x4*)(p.part_o + at * D + d4) = x;
-      if (d4 == 0) {
-        p.part_ml[2 * at] = m;
-        p.part_ml[2 * at + 1] = l;
+          for (int g = 0; g < 4; ++g)
+            if (mine) *(f32x4*)(p.part_o + part * D + 32 * a + 8 * g + 4 * hl) =
+                f32x4{acc[a][4 * g], acc[a][4 * g + 1], acc[a][4 * g + 2], acc[a][4 * g + 3]};
+        if (mine && hl == 0) {
+          p.part_ml[2 * part] = m_run;
+          p.part_ml[2 * part + 1] = l;
+        }
       }
+      m_run = kPagedNoMax;
+      l_run = 0.f;
+      row_wrong = false;
+      begun = true;
+#pragma unroll
+      for (int a = 0; a < NA; ++a) acc[a] = f32x16{};
     }
+    if (i + 1 < n) advance(at);
   }
 }
 
-// o of one (sequence, head) from its workgroups' parts: D / 4 lanes a row, the parts in their order.
+// o of one (sequence, query head) that several waves hold: D / 4 lanes a part, 256 / (D / 4) parts side by side, each group
+// with a running maximum over its own, then the groups in LDS in their order.
 template <bool F16, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   using T = typename Elem<F16>::T;
-  constexpr int TPR = D / 4;
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x, row = gid / TPR;
-  const int d4 = (int)(gid % TPR) * 4;
-  if (row >= (int64_t)p.batch * p.heads) return;
-  const int b = (int)(row / p.heads), h = (int)(row % p.heads);
-  bool bad;
-  const int len = paged_length(p, b, bad);
-  const int n = bad ? 1 : max(1, (len + p.chunk - 1) / p.chunk);
-  float m = kPagedNoMax, l = 0.f;
-  for (int s = 0; s < n; ++s) m = fmaxf(m, p.part_ml[2 * (row * p.chunks + s)]);
-  f32x4 x = f32x4{};
-  for (int s = 0; s < n; ++s) {
-    const int64_t at = row * p.chunks + s;
-    const float f = fast_exp2(p.part_ml[2 * at] - m);
-    l = fmaf(p.part_ml[2 * at + 1], f, l);
-    const f32x4 y = *(const f32x4*)(p.part_o + at * D + d4);
+  constexpr int TPR = D / 4, NG = 256 / TPR;
+  __shared__ float sums[NG][D], ml[NG][2];
+  __shared__ int64_t wave_sums[4][2];
+  const int tid = threadIdx.x, b = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
+  const int kvh = h / p.group, in = h % p.group, x = kvh * p.blocks + in / p.per, X = p.kv_heads * p.blocks;
+  int64_t all = 0, before = 0;   // tiles of all sequences, and of those before b
+  for (int s = tid; s < p.batch; s += 256) {
+    const int t = paged_seq(p, p.lengths[s]).tiles;
+    all += t;
+    before += s < b ? t : 0;
+  }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = fmaf(y[e], f, x[e]);
+  for (int m = 32; m >= 1; m >>= 1) {
+    all += __shfl_xor(all, m);
+    before += __shfl_xor(before, m);
+  }
+  if ((tid & 63) == 0) {
+    wave_sums[tid >> 6][0] = all;
+    wave_sums[tid >> 6][1] = before;
+  }
+  __syncthreads();
+  all = before = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    all += wave_sums[i][0];
+    before += wave_sums[i][1];
+  }
+  const int tiles = paged_seq(p, p.lengths[b]).tiles;
+  const int64_t total = all * X, W = p.waves < total ? p.waves : total, t0 = before * X + (int64_t)x * tiles;
+  const int64_t w0 = paged_owner(t0, W, total), w1 = paged_owner(t0 + tiles - 1, W, total);
+  if (w0 == w1) return;   // one wave had it all
+  const int g = tid / TPR, d4 = (tid % TPR) * 4;
+  float m = kPagedNoMax, l = 0.f;
+  f32x4 acc = f32x4{};
+  for (int64_t w = w0 + g; w <= w1; w += NG) {
+    const int64_t part = (w + (int64_t)b * X + x) * p.per + in % p.per;
+    const float pm = p.part_ml[2 * part], pl = p.part_ml[2 * part + 1];
+    const f32x4 y = *(const f32x4*)(p.part_o + part * D + d4);
+    const float m_new = fmaxf(m, pm), f = fast_exp2(m - m_new), pf = fast_exp2(pm - m_new);
+    m = m_new;
+    l = fmaf(l, f, pl * pf);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(acc[e], f, y[e] * pf);
+  }
+  *(f32x4*)&sums[g][d4] = acc;
+  if (d4 == 0) {
+    ml[g][0] = m;
+    ml[g][1] = l;
+  }
+  __syncthreads();
+  if (g > 0) return;
+  m = kPagedNoMax;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < NG; ++i) m = fmaxf(m, ml[i][0]);
+  acc = f32x4{};
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    const float f = fast_exp2(ml[i][0] - m);
+    l = fmaf(ml[i][1], f, l);
+    const f32x4 y = *(const f32x4*)&sums[i][d4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(y[e], f, acc[e]);
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   typename Elem<F16>::V4 y;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = to_elem<T>(x[e] * inv);
+  for (int e = 0; e < 4; ++e) y[e] = to_elem<T>(acc[e] * inv);
   *(typename Elem<F16>::V4*)((T*)p.o + (int64_t)b * p.o_sb + (int64_t)h * p.o_sh + d4) = y;
 }
 
@@ -299,29 +435,27 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(CopyParams p) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
-// Keys a workgroup takes: long chunks keep its start and its join small beside the keys, but at the table's width there
-// should be workgroups for four rounds of the chip's 256 CUs.
-static int paged_chunk(const vmo_paged_args* a) {
-  const int64_t most = (int64_t)a->table_width * a->page_size;
-  const int64_t rows = (int64_t)a->batch * a->kv_heads;
-  int64_t chunk = (most * rows + 1023) / 1024;
-  chunk = (chunk + 127) / 128 * 128;
-  return (int)(chunk < 128 ? 128 : chunk > kPagedMaxChunk ? kPagedMaxChunk : chunk);
+// Waves of a launch: as many as the chip holds at once (256 CUs of 160 KB LDS), one round.  LDS of a wave: two K and two V
+// tiles, four slots of its group's queries.
+struct PagedShape { int blocks, per, q_rows, lds, waves; };
+static PagedShape paged_shape(const vmo_paged_args* a) {
+  PagedShape s;
+  const int group = a->heads / a->kv_heads, rpi = 512 / a->d;
+  s.blocks = (group + 31) / 32;
+  s.per = (group + s.blocks - 1) / s.blocks;
+  s.q_rows = (s.per + rpi - 1) / rpi * rpi;
+  s.lds = 4 * kPagedTile * a->d * 2 + 4 * s.q_rows * a->d * 2;
+  const int fit = 160 * 1024 / s.lds;
+  s.waves = 256 * (fit < 8 ? fit : 8);
+  return s;
 }
 
 template <bool F16, int D>
-static int launch_paged(const PagedParams& p, hipStream_t s) {
-  constexpr int RING = kPagedWaves * 2 * 2 * kPagedTile * D * 2, LDS = RING + kPagedMaxChunk * 4 / 8;
-  static_assert(1024 + kPagedWaves * 32 * (D + 4) * 4 <= RING + 2048, "the join fits the ring");
-  auto kern = paged_attention_kernel<F16, D>;
-  if (LDS > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
-    return set_error(VMO_ERR_LAUNCH, "paged_attention: cannot raise the LDS limit to %d bytes", LDS);
-  const dim3 grid((unsigned)((int64_t)p.batch * p.kv_heads * p.chunks), (unsigned)((p.group + 31) / 32));
-  hipLaunchKernelGGL(kern, grid, dim3(64 * kPagedWaves), LDS, s, p);
+static int launch_paged(const PagedParams& p, int lds, hipStream_t s) {
+  hipLaunchKernelGGL((paged_attention_kernel<F16, D>), dim3((unsigned)p.waves), dim3(64), lds, s, p);
   const int rc = launch_status("paged_attention");
-  if (rc != VMO_OK || p.chunks == 1) return rc;
-  const int64_t threads = (int64_t)p.batch * p.heads * (D / 4);
-  hipLaunchKernelGGL((paged_join_kernel<F16, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
+  if (rc != VMO_OK) return rc;
+  hipLaunchKernelGGL((paged_join_kernel<F16, D>), dim3((unsigned)(p.batch * p.heads)), dim3(256), 0, s, p);
   return launch_status("paged_join");
 }
 
@@ -335,10 +469,9 @@ static bool page_size_ok(int n) { return n >= 8 && n <= 1024 && (n & (n - 1)) ==
 }  // namespace vmo
 
 extern "C" size_t vmo_paged_attention_workspace_size(const vmo_paged_args* a) {
-  if (!a || a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->table_width <= 0 || a->page_size <= 0 || a->d <= 0) return 0;
-  const int chunk = vmo::paged_chunk(a);
-  const int64_t chunks = ((int64_t)a->table_width * a->page_size + chunk - 1) / chunk;
-  return chunks <= 1 ? 0 : (size_t)((int64_t)a->batch * a->heads * chunks * (a->d + 2) * 4);
+  if (!a || a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || (a->d != 64 && a->d != 128)) return 0;
+  const vmo::PagedShape s = vmo::paged_shape(a);
+  return (size_t)((s.waves + (int64_t)a->batch * a->kv_heads * s.blocks) * s.per * (a->d + 2) * 4);
 }
 
 extern "C" int vmo_paged_attention(const vmo_paged_args* a, void* stream) {
@@ -352,13 +485,15 @@ extern "C" int vmo_paged_attention(const vmo_paged_args* a, void* stream) {
   if (!page_size_ok(a->page_size))
     return set_error(VMO_ERR_UNSUPPORTED, "paged_attention: pages of %d tokens (powers of two from 8 to 1024)", a->page_size);
   if (a->batch == 0) return VMO_OK;
-  if (a->pages < 1 || a->table_width < 1 || (int64_t)a->table_width * a->page_size > (1ll << 30) ||
+  if (a->pages < 1 || a->table_width < 1 || (int64_t)a->table_width * a->page_size > (1ll << 28) ||
       (int64_t)a->batch * a->heads > (1ll << 30))
     return set_error(VMO_ERR_INVALID, "paged_attention: %d pages, %d page numbers a sequence", a->pages, a->table_width);
   if (!a->table || !a->lengths) return set_error(VMO_ERR_INVALID, "paged_attention: no page table or lengths");
   if (!view_ok(a->k) || !view_ok(a->v) || !a->q.data || !a->o.data || !aligned16(a->q.data) || !aligned16(a->o.data) ||
       a->q.stride_b % 8 || a->q.stride_h % 8 || a->o.stride_b % 8 || a->o.stride_h % 8)
     return set_error(VMO_ERR_INVALID, "paged_attention: tensors need 16-byte aligned rows (strides multiple of 8 elements)");
+  if (a->k.stride_n >= (1ll << 27) || a->v.stride_n >= (1ll << 27))   // (32-bit lane offsets over up to 7 rows)
+    return set_error(VMO_ERR_UNSUPPORTED, "paged_attention: token stride must be below 2^27 elements");
   if (!(a->sm_scale >= 0.f) || a->sm_scale > 3.0e38f)
     return set_error(VMO_ERR_INVALID, "paged_attention: sm_scale must be finite and >= 0");
   PagedParams p{};
@@ -369,21 +504,19 @@ extern "C" int vmo_paged_attention(const vmo_paged_args* a, void* stream) {
   p.table = a->table; p.lengths = a->lengths; p.t_sb = a->table_stride;
   p.batch = a->batch; p.heads = a->heads; p.kv_heads = a->kv_heads; p.group = a->heads / a->kv_heads;
   p.pages = a->pages; p.page_log = log2_of(a->page_size); p.width = a->table_width;
-  p.chunk = paged_chunk(a);
-  const int64_t chunks = ((int64_t)a->table_width * a->page_size + p.chunk - 1) / p.chunk;
-  if ((int64_t)a->batch * a->kv_heads * chunks > (1ll << 30)) return set_error(VMO_ERR_UNSUPPORTED, "paged_attention: batch too large");
-  p.chunks = (int)chunks;
+  const PagedShape shape = paged_shape(a);
+  p.blocks = shape.blocks; p.per = shape.per; p.q_rows = shape.q_rows; p.waves = shape.waves;
   const size_t need = vmo_paged_attention_workspace_size(a);
   if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)))
     return set_error(VMO_ERR_WORKSPACE, "paged_attention: needs %llu workspace bytes, has %llu", (unsigned long long)need,
                      (unsigned long long)(a->workspace ? a->workspace_bytes : 0));
   p.part_o = (float*)a->workspace;
-  p.part_ml = p.part_o + (int64_t)a->batch * a->heads * chunks * a->d;
+  p.part_ml = p.part_o + (p.waves + (int64_t)a->batch * a->kv_heads * p.blocks) * p.per * a->d;
   p.c = a->sm_scale * kLog2e;
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = a->dtype == VMO_DTYPE_F16;
-  if (a->d == 64) return f16 ? launch_paged<true, 64>(p, s) : launch_paged<false, 64>(p, s);
-  return f16 ? launch_paged<true, 128>(p, s) : launch_paged<false, 128>(p, s);
+  if (a->d == 64) return f16 ? launch_paged<true, 64>(p, shape.lds, s) : launch_paged<false, 64>(p, shape.lds, s);
+  return f16 ? launch_paged<true, 128>(p, shape.lds, s) : launch_paged<false, 128>(p, shape.lds, s);
 }
 
 extern "C" int vmo_append_pages(const vmo_append_args* a, void* stream) {
