@@ -43,10 +43,11 @@ __device__ __forceinline__ int64_t paged_owner(int64_t tile, int64_t waves, int6
 // ------------------------------------------------------------------------------------------------
 // A wave is a workgroup of its own and walks its share of the tiles, over the ends of sequences: 32 keys of one key / value
 // head against the query heads of its group, the columns of the 32-wide products (S^T = K Q^T, O^T += V^T P^T, a lane one
-// query head, as in the forward of whole prompts).  K and V tiles have two LDS slots each; K of tile i + 2 is fetched when
-// S of tile i is formed, V of it when P V is, so three quarters of the wave's LDS is always under way, and no barrier is
-// met.  Page numbers and lengths come through the scalar unit, whose waits leave the copies alone; a copy instruction lies
-// within one page (pages hold 8 tokens at least), so its address is scalar too.
+// query head, as in the forward of whole prompts).  Two LDS slots take a tile's K and V; once tile i has landed it goes to
+// registers whole and tile i + 2 is fetched into its place before anything is computed, so that the copies of two tiles
+// are under way all the time (24 KB a wave with K and V held in LDS through their products, 32 KB so: 64 sequences of 84k
+// tokens, 8 heads of 128 @@), and no barrier is met.  Page numbers and lengths come through the scalar unit, whose waits
+// leave the copies alone; a copy instruction lies within one page (pages hold 8 tokens at least), so its address is scalar.
 // Bound by the bytes of the cache, 2 D 2 a key and head, and by how many of them are in flight.
 template <bool F16, int D>
 __global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams p) {
@@ -113,57 +114,58 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams p) {
     koff[j] = (uint32_t)((lane / CH) * p.k_sn * 2) + chunk;
     voff[j] = (uint32_t)((lane / CH) * p.v_sn * 2) + chunk;
   }
-  // The tile under `next`: its page numbers, then K (with the row's queries where it begins one, or the wave does), then V.
-  // ids[j]: the page of rows 8 j .. 8 j + 7.  A number outside the cache is not followed: page 0 instead, and the row is
-  // marked (bit i % 4 of `wrong`).
+  // The tile under `next`.  Its page numbers (raw[j]: rows 8 j .. 8 j + 7) are asked for when the tile before is issued.  A
+  // number outside the cache is not followed: page 0 instead, and the row is marked (bit i % 4 of `wrong`).  Offsets within
+  // a page have 32 bits, and so have page strides in bytes.
   Cursor next = at;
-  int ids[4];
+  int raw[4];
   uint32_t wrong = 0;
   const int place_mask = (1 << p.page_log) - 1;
-  auto pages_of_tile = [&](int i) __attribute__((always_inline)) {
-    const int64_t row = next.b * p.t_sb;
-    const int key0 = next.tile * kPagedTile, last = (next.s.len - 1) >> p.page_log;
-    bool bad = next.s.bad;
+  const uint32_t k_row = (uint32_t)p.k_sn * 2, v_row = (uint32_t)p.v_sn * 2, k_page = (uint32_t)(p.k_sp * 2), v_page = (uint32_t)(p.v_sp * 2);
+  auto ask_pages = [&]() __attribute__((always_inline)) {
+    // (a sequence without tokens reads its first place, which the table has)
+    const int first_page = (next.tile * kPagedTile) >> p.page_log, last = max((next.s.len - 1) >> p.page_log, 0);
+    const scalar_ints row = table + next.b * p.t_sb;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int page = min((key0 + 8 * j) >> p.page_log, last);
-      int id = 0;
-      if (next.s.len > 0) id = table[row + page];
-      const bool out = id < 0 || id >= p.pages;
-      bad |= out;
-      ids[j] = out ? 0 : id;
-    }
-    wrong = (wrong & ~(1u << (i & 3))) | (bad ? 1u << (i & 3) : 0u);
-  };
-  auto copy_tile = [&](const void* base, int64_t sp, int64_t sh, int64_t sn, const uint32_t (&off)[NV], uint32_t dst)
-      __attribute__((always_inline)) {
-    const uint64_t head = (uint64_t)(uintptr_t)base + (uint64_t)((next.x / p.blocks) * sh * 2);
-    const int key0 = next.tile * kPagedTile;
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int r = j * RPI;
-      dma16_async_s(head + (uint64_t)(ids[r / 8] * sp + ((key0 + r) & place_mask) * sn) * 2, off[j % NV], dst + j * 1024);
-    }
+    for (int j = 0; j < 4; ++j) raw[j] = row[min(first_page + ((8 * j) >> p.page_log), last)];
   };
   const uint32_t q_slots = lds + 4 * UNIT;
   const int slot_bytes = p.q_rows * RB;
-  auto issue_k = [&](int i) __attribute__((always_inline)) {
-    pages_of_tile(i);
-    if (next.tile == 0 || i == 0) {
-      const int h0 = (next.x / p.blocks) * p.group + (next.x % p.blocks) * p.per, most = min(p.per, p.group - (next.x % p.blocks) * p.per) - 1;
+  auto issue = [&](int i) __attribute__((always_inline)) {
+    const int kvh = next.x / p.blocks;
+    if (next.tile == 0 || i == 0) {   // the row's queries too
+      const int h0 = kvh * p.group + (next.x % p.blocks) * p.per, most = min(p.per, p.group - (next.x % p.blocks) * p.per) - 1;
       for (int r = 0; r < p.q_rows; r += RPI)
         dma16_async((const T*)p.q + next.b * p.q_sb + (h0 + min(r + lane / CH, most)) * p.q_sh + (lane % CH) * 8,
                     q_slots + (i & 3) * slot_bytes + r * RB);
     }
-    copy_tile(p.k, p.k_sp, p.k_sh, p.k_sn, koff, lds + (i & 1) * 2 * UNIT);
-  };
-  auto issue_v = [&](int i) __attribute__((always_inline)) {
-    copy_tile(p.v, p.v_sp, p.v_sh, p.v_sn, voff, lds + (i & 1) * 2 * UNIT + UNIT);
-    if (i + 1 < n) advance(next);
-  };
-  // waits until all but the newest `units` K or V tiles have landed
-  auto landed = [&](auto units) __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(decltype(units)::value * NI) : "memory");
+    bool bad = next.s.bad;
+    uint32_t id[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool out = (uint32_t)raw[j] >= (uint32_t)p.pages;
+      bad |= out && next.s.len > 0;
+      id[j] = out ? 0 : raw[j];
+    }
+    wrong = (wrong & ~(1u << (i & 3))) | (bad ? 1u << (i & 3) : 0u);
+    const uint32_t key0 = next.tile * kPagedTile, dst = lds + (i & 1) * 2 * UNIT;
+    auto copy_tile = [&](const void* base, int64_t sh, uint32_t page, uint32_t row, const uint32_t (&off)[NV], uint32_t to)
+        __attribute__((always_inline)) {
+      const uint64_t head = (uint64_t)(uintptr_t)base + (uint64_t)(kvh * sh * 2) + (uint64_t)((key0 & place_mask) * row);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t at8 = head + (uint64_t)id[j] * page + (uint64_t)(((8 * j) & place_mask) * row);
+#pragma unroll
+        for (int h = 0; h < 8 / RPI; ++h)
+          dma16_async_s(at8 + (uint64_t)(h * RPI) * row, off[(j * (8 / RPI) + h) % NV], to + (j * (8 / RPI) + h) * 1024);
+      }
+    };
+    copy_tile(p.k, p.k_sh, k_page, k_row, koff, dst);
+    copy_tile(p.v, p.v_sh, v_page, v_row, voff, dst + UNIT);
+    if (i + 1 < n) {
+      advance(next);
+      ask_pages();
+    }
   };
   auto reads_done = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); };
 
@@ -177,16 +179,13 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams p) {
   const int trow = 4 * hl + ((lane & 15) >> 2), tchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), tbyte = (lane & 1) * 8;
   bool begun = at.tile == 0, row_wrong = false;   // whether the wave has the row from its first tile
 
-  issue_k(0);
-  issue_v(0);
-  if (n > 1) {
-    issue_k(1);
-    issue_v(1);
-  }
+  ask_pages();
+  issue(0);
+  if (n > 1) issue(1);
   for (int i = 0; i < n; ++i) {
-    const VMO_LDS char* Ks = smem + (i & 1) * 2 * UNIT;
-    if (i + 1 < n) landed(std::integral_constant<int, 3>{});
-    else landed(std::integral_constant<int, 1>{});
+    VMO_LDS char* Ks = smem + (i & 1) * 2 * UNIT;
+    if (i + 1 < n) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * NI) : "memory");   // all but tile i + 1 has landed
+    else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     const int nh = min(p.per, p.group - (at.x % p.blocks) * p.per);
     if (at.tile == 0 || i == 0) {
       const VMO_LDS char* qs = smem + 4 * UNIT + (i & 3) * slot_bytes + min(l32, nh - 1) * RB + hl * 16;
@@ -194,13 +193,28 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams p) {
       for (int ds = 0; ds < NDS; ++ds) qf[ds] = lds_read8<V8>(qs + ds * 32);
     }
     row_wrong |= (wrong >> (i & 3)) & 1;
+    const int nvis = at.s.len - at.tile * kPagedTile;   // keys of the tile that there are
+    if (nvis < kPagedTile) {   // places without a token hold anything: 0 times that need not be 0
+      const int gone = max(nvis, 0);
+      for (int j = lane; j < (kPagedTile - gone) * CH; j += 64) *(VMO_LDS f32x4*)(Ks + UNIT + gone * RB + j * 16) = f32x4{};
+      reads_done();
+    }
+    // the whole tile into registers, so that its slots can be filled again before anything is computed
+    V8 kf[NDS], vf[2 * NA];
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) kf[ds] = lds_read8<V8>(Ks + l32 * RB + ((2 * ds + hl) ^ sw) * 16);
+#pragma unroll
+    for (int j = 0; j < 2 * NA; ++j) {
+      const int c0 = trow * RB + (((4 * (j / 2) + tchunk) ^ swz_rows<RB>(trow)) * 16 + tbyte);
+      const VMO_LDS char* rp = Ks + UNIT + 16 * (j % 2) * RB;
+      vf[j] = lds_read_tr8<V8>(rp + c0, rp + 8 * RB + (c0 ^ 32));
+    }
+    reads_done();
+    if (i + 2 < n) issue(i + 2);
+
     f32x16 s = f32x16{};
 #pragma unroll
-    for (int ds = 0; ds < NDS; ++ds) s = E::mfma(lds_read8<V8>(Ks + l32 * RB + ((2 * ds + hl) ^ sw) * 16), qf[ds], s);
-    reads_done();
-    if (i + 2 < n) issue_k(i + 2);
-
-    const int nvis = at.s.len - at.tile * kPagedTile;   // keys of the tile that there are
+    for (int ds = 0; ds < NDS; ++ds) s = E::mfma(kf[ds], qf[ds], s);
     V8 P[2];
     auto weights = [&]() __attribute__((always_inline)) {
       float ls = 0.f;
@@ -232,26 +246,8 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams p) {
     }
     l_run += ls;
 
-    if (i + 2 < n) landed(std::integral_constant<int, 3>{});
-    else if (i + 1 < n) landed(std::integral_constant<int, 2>{});
-    else landed(std::integral_constant<int, 0>{});
-    if (nvis < kPagedTile) {   // places without a token hold anything: 0 times that need not be 0
-      const int gone = max(nvis, 0);
-      for (int j = lane; j < (kPagedTile - gone) * CH; j += 64)
-        *(VMO_LDS f32x4*)(smem + (i & 1) * 2 * UNIT + UNIT + gone * RB + j * 16) = f32x4{};
-      reads_done();
-    }
 #pragma unroll
-    for (int a = 0; a < NA; ++a) {
-      const int c0 = trow * RB + (((4 * a + tchunk) ^ swz_rows<RB>(trow)) * 16 + tbyte);
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        const VMO_LDS char* rp = Ks + UNIT + 16 * h2 * RB;
-        acc[a] = E::mfma(lds_read_tr8<V8>(rp + c0, rp + 8 * RB + (c0 ^ 32)), P[h2], acc[a]);
-      }
-    }
-    reads_done();
-    if (i + 2 < n) issue_v(i + 2);
+    for (int j = 0; j < 2 * NA; ++j) acc[j / 2] = E::mfma(vf[j], P[j % 2], acc[j / 2]);
 
     const bool ends = at.tile + 1 == at.s.tiles;
     if (ends || i + 1 == n) {   // the row is done here: whole, or this wave's part of it
@@ -494,6 +490,9 @@ extern "C" int vmo_paged_attention(const vmo_paged_args* a, void* stream) {
     return set_error(VMO_ERR_INVALID, "paged_attention: tensors need 16-byte aligned rows (strides multiple of 8 elements)");
   if (a->k.stride_n >= (1ll << 27) || a->v.stride_n >= (1ll << 27))   // (32-bit lane offsets over up to 7 rows)
     return set_error(VMO_ERR_UNSUPPORTED, "paged_attention: token stride must be below 2^27 elements");
+  for (const vmo_view* x : {&a->k, &a->v})   // offsets within a page, and page strides, in 32 bits of bytes
+    if (x->stride_b < 0 || x->stride_b >= (1ll << 31) || x->stride_n * a->page_size >= (1ll << 30))
+      return set_error(VMO_ERR_UNSUPPORTED, "paged_attention: pages must be below 2^31 elements apart, a head of one below 2^30 long");
   if (!(a->sm_scale >= 0.f) || a->sm_scale > 3.0e38f)
     return set_error(VMO_ERR_INVALID, "paged_attention: sm_scale must be finite and >= 0");
   PagedParams p{};
