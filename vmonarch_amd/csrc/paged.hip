@@ -22,6 +22,7 @@ struct PagedParams {
   int blocks, per;           // a sequence's rows: kv_heads x blocks of `per` (at most 32) query heads
   int waves, q_rows;         // waves launched; query rows that an LDS slot holds (per, in whole copies)
   float *part_o, *part_ml;   // (waves + batch kv_heads blocks) parts of (per, D), and of (per, 2): sums, then m and l
+  int* starts;
   float c;
 };
 
@@ -35,10 +36,11 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int len) {
   s.tiles = max((s.len + kPagedTile - 1) / kPagedTile, 1);
   return s;
 }
-// Tiles of all rows stand in one order (sequence, row of it, tile); wave w of W takes those from w total / W up to
-// (w + 1) total / W, so tile T belongs to wave ((T + 1) W - 1) / total.  A row that several waves hold has a part from each,
-// in place (wave + row): along the order one of the two grows with every part, so places are its own.
-__device__ __forceinline__ int64_t paged_owner(int64_t tile, int64_t waves, int64_t total) { return ((tile + 1) * waves - 1) / total; }
+// Tiles of all rows stand in one order (sequence, row of it, tile) and are dealt to the waves in equal shares of their
+// cost: a tile counts 1, a row's begin and end c more (1 where a wave has two tiles at least: 64 sequences of 16 to 8192
+// tokens, 8 heads of 128, @@ with it, whose short rows would otherwise end up with a few waves).  A row that several waves
+// hold has a part from each, in place (wave + row): along the order one of the two grows with every part, so places are its
+// own.  starts[w]: the row that wave w begins inside of, or -1.
 
 // ------------------------------------------------------------------------------------------------
 // A wave is a workgroup of its own and walks its share of the tiles, over the ends of sequences: 32 keys of one key / value
@@ -66,36 +68,68 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams p) {
   const scalar_ints lengths = (scalar_ints)(uintptr_t)p.lengths, table = (scalar_ints)(uintptr_t)p.table;
   const int X = p.kv_heads * p.blocks;   // rows of a sequence
 
-  // this wave's tiles
-  int64_t sum = 0;
-  for (int b = lane; b < p.batch; b += 64) sum += paged_seq(p, p.lengths[b]).tiles;
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
-  const int64_t total = uniform64((uint64_t)sum) * X;
-  const int64_t W = p.waves < total ? p.waves : total, w = blockIdx.x;
-  if (w >= W) return;
-  const int64_t first = w * total / W;
-  const int n = (int)((w + 1) * total / W - first);
-  int b = 0;
-  int64_t before = 0;   // tiles of the sequences before b, of one row
-  for (int s0 = 0;; s0 += 64) {
-    const int tiles = s0 + lane < p.batch ? paged_seq(p, p.lengths[s0 + lane]).tiles : 0;
-    const int upto = wave_scan_i32(tiles), all = __builtin_amdgcn_readlane(upto, 63);
-    if ((before + all) * X > first) {
-      const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64((before + upto) * X > first));
-      b = s0 + who;
-      before += __builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(tiles, who);
-      break;
+  // this wave's tiles: sums of 64 sequences each wait in LDS, then the sequence that holds a position of the order
+  // (the first 64, often all, stay in registers)
+  auto tiles_of = [&](int at, int len) __attribute__((always_inline)) { return at < p.batch ? paged_seq(p, len).tiles : 0; };
+  auto length_at = [&](int at) __attribute__((always_inline)) { return p.lengths[min(at, p.batch - 1)]; };
+  VMO_LDS int* sums = (VMO_LDS int*)smem;
+  const int n_sums = (p.batch + 63) / 64;
+  const int len0 = length_at(lane), tiles0 = tiles_of(lane, len0), upto0 = wave_scan_i32(tiles0);
+  int64_t all = __builtin_amdgcn_readlane(upto0, 63);
+  if (n_sums > 1) {
+    if (lane == 0) sums[0] = (int)all;
+#pragma unroll 4
+    for (int i = 1; i < n_sums; ++i) {
+      const int t = wave_sum_i32(tiles_of(i * 64 + lane, length_at(i * 64 + lane)));
+      if (lane == 0) sums[i] = t;
+      all += t;
     }
-    before += all;
   }
+  // 64-bit division is long: 32 bits where both fit
+  auto quotient = [](int64_t a, int64_t b) __attribute__((always_inline)) {
+    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+  };
+  const int c_row = all * X >= 2 * (int64_t)p.waves ? 1 : 0;
+  const int64_t total = (all + (int64_t)c_row * p.batch) * X, W = p.waves < total ? p.waves : total, w = blockIdx.x;
+  if (w >= W) {
+    if (lane == 0) p.starts[w] = -1;
+    return;
+  }
+  struct Place { int b, x, tile, len; int64_t tiles; };   // tiles: of all rows before it
+  auto place_of = [&](int64_t pos) __attribute__((always_inline)) {
+    Place r;
+    int64_t before = 0;   // tiles of the sequences before, of one row
+    int i = 0;
+    while (i + 1 < n_sums && (before + sums[i] + (int64_t)c_row * 64 * (i + 1)) * X <= pos) before += sums[i++];
+    int len = len0, tiles = tiles0, upto = upto0;
+    if (i > 0) {
+      len = length_at(i * 64 + lane);
+      tiles = tiles_of(i * 64 + lane, len);
+      upto = wave_scan_i32(tiles);
+    }
+    const uint64_t over = __builtin_amdgcn_ballot_w64((before + upto + (int64_t)c_row * (i * 64 + lane + 1)) * X > pos);
+    const int who = over ? __builtin_ctzll(over) : min(63, p.batch - 1 - i * 64);   // (none: the end of the last sequence)
+    const int mine = __builtin_amdgcn_readlane(tiles, who);
+    r.b = __builtin_amdgcn_readfirstlane(i * 64 + who);
+    r.len = __builtin_amdgcn_readlane(len, who);
+    before += __builtin_amdgcn_readlane(upto, who) - mine;
+    const int64_t rest = pos - (before + (int64_t)c_row * r.b) * X;
+    r.x = (int)quotient(rest, mine + c_row);
+    r.tile = max((int)(rest - (int64_t)r.x * (mine + c_row)) - c_row, 0);
+    r.tiles = before * X + (int64_t)r.x * mine + r.tile;
+    return r;
+  };
+  const Place from = place_of(quotient(w * total, W)), to = place_of(quotient((w + 1) * total, W));
+  const int n = (int)(to.tiles - from.tiles);
+  if (lane == 0) p.starts[w] = from.tile > 0 ? from.b * X + from.x : -1;
+  if (n <= 0) return;
+  __syncthreads();   // (one wave: its LDS reads are done before the copies come)
   struct Cursor { int b, x, tile; PagedSeq s; };   // row x of sequence b, its tile
   Cursor at;
-  at.b = uni(b);
-  at.s = paged_seq(p, lengths[at.b]);
-  const int64_t rest = first - before * X;
-  at.x = uni((int)(rest / at.s.tiles));
-  at.tile = uni((int)(rest % at.s.tiles));
+  at.b = uni(from.b);
+  at.x = uni(from.x);
+  at.tile = uni(from.tile);
+  at.s = paged_seq(p, uni(from.len));
   auto advance = [&](Cursor& c) __attribute__((always_inline)) {
     if (++c.tile < c.s.tiles) return;
     c.tile = 0;
@@ -290,47 +324,41 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams p) {
   }
 }
 
-// o of one (sequence, query head) that several waves hold: D / 4 lanes a part, 256 / (D / 4) parts side by side, each group
-// with a running maximum over its own, then the groups in LDS in their order.
+// o of a row that several waves hold, one query head a workgroup: the workgroup of the first wave that begins inside it.
+// D / 4 lanes a part, 256 / (D / 4) parts side by side, each group with a running maximum over its own, then the groups in
+// LDS in their order.  Bound by the latency of three reads in a row (starts, starts of the waves behind, parts).
 template <bool F16, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   using T = typename Elem<F16>::T;
   constexpr int TPR = D / 4, NG = 256 / TPR;
   __shared__ float sums[NG][D], ml[NG][2];
-  __shared__ int64_t wave_sums[4][2];
-  const int tid = threadIdx.x, b = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
-  const int kvh = h / p.group, in = h % p.group, x = kvh * p.blocks + in / p.per, X = p.kv_heads * p.blocks;
-  int64_t all = 0, before = 0;   // tiles of all sequences, and of those before b
-  for (int s = tid; s < p.batch; s += 256) {
-    const int t = paged_seq(p, p.lengths[s]).tiles;
-    all += t;
-    before += s < b ? t : 0;
-  }
+  const int w = blockIdx.x, in = blockIdx.y, tid = threadIdx.x;
+  const int row = p.starts[w], last = w > 0 ? p.starts[w - 1] : -1;
+  if (row < 0 || row == last) return;
+  const int X = p.kv_heads * p.blocks, b = row / X, x = row % X, block = x % p.blocks;
+  if (in >= min(p.per, p.group - block * p.per)) return;
+  const int h = (x / p.blocks) * p.group + block * p.per + in;
+  // waves w .. w + more - 1 begin inside the row; wave w - 1 has its first tiles
+  __shared__ int firsts[4];
+  int more = 0;
+  for (bool on = true; on; ) {
+    const int v = w + more + tid;
+    const uint64_t out = __builtin_amdgcn_ballot_w64(v >= p.waves || p.starts[min(v, p.waves - 1)] != row);
+    if ((tid & 63) == 0) firsts[tid >> 6] = out ? __builtin_ctzll(out) : 64;
+    __syncthreads();
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    all += __shfl_xor(all, m);
-    before += __shfl_xor(before, m);
+    for (int i = 0; i < 4; ++i) {
+      if (on) more += firsts[i];
+      on = on && firsts[i] == 64;
+    }
+    __syncthreads();
   }
-  if ((tid & 63) == 0) {
-    wave_sums[tid >> 6][0] = all;
-    wave_sums[tid >> 6][1] = before;
-  }
-  __syncthreads();
-  all = before = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    all += wave_sums[i][0];
-    before += wave_sums[i][1];
-  }
-  const int tiles = paged_seq(p, p.lengths[b]).tiles;
-  const int64_t total = all * X, W = p.waves < total ? p.waves : total, t0 = before * X + (int64_t)x * tiles;
-  const int64_t w0 = paged_owner(t0, W, total), w1 = paged_owner(t0 + tiles - 1, W, total);
-  if (w0 == w1) return;   // one wave had it all
   const int g = tid / TPR, d4 = (tid % TPR) * 4;
   float m = kPagedNoMax, l = 0.f;
   f32x4 acc = f32x4{};
-  for (int64_t w = w0 + g; w <= w1; w += NG) {
-    const int64_t part = (w + (int64_t)b * X + x) * p.per + in % p.per;
+#pragma unroll 4
+  for (int v = g; v <= more; v += NG) {
+    const int64_t part = (w - 1 + v + (int64_t)row) * p.per + in;
     const float pm = p.part_ml[2 * part], pl = p.part_ml[2 * part + 1];
     const f32x4 y = *(const f32x4*)(p.part_o + part * D + d4);
     const float m_new = fmaxf(m, pm), f = fast_exp2(m - m_new), pf = fast_exp2(pm - m_new);
@@ -443,6 +471,9 @@ static PagedShape paged_shape(const vmo_paged_args* a) {
   s.lds = 4 * kPagedTile * a->d * 2 + 4 * s.q_rows * a->d * 2;
   const int fit = 160 * 1024 / s.lds;
   s.waves = 256 * (fit < 8 ? fit : 8);
+  // no more than the tiles that the table has room for
+  const int64_t most = (int64_t)a->batch * a->kv_heads * s.blocks * (((int64_t)a->table_width * a->page_size + kPagedTile - 1) / kPagedTile);
+  if (most < s.waves) s.waves = most < 1 ? 1 : (int)most;
   return s;
 }
 
@@ -451,7 +482,7 @@ static int launch_paged(const PagedParams& p, int lds, hipStream_t s) {
   hipLaunchKernelGGL((paged_attention_kernel<F16, D>), dim3((unsigned)p.waves), dim3(64), lds, s, p);
   const int rc = launch_status("paged_attention");
   if (rc != VMO_OK) return rc;
-  hipLaunchKernelGGL((paged_join_kernel<F16, D>), dim3((unsigned)(p.batch * p.heads)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((paged_join_kernel<F16, D>), dim3((unsigned)p.waves, (unsigned)p.per), dim3(256), 0, s, p);
   return launch_status("paged_join");
 }
 
@@ -465,9 +496,11 @@ static bool page_size_ok(int n) { return n >= 8 && n <= 1024 && (n & (n - 1)) ==
 }  // namespace vmo
 
 extern "C" size_t vmo_paged_attention_workspace_size(const vmo_paged_args* a) {
-  if (!a || a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || (a->d != 64 && a->d != 128)) return 0;
+  if (!a || a->batch <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->heads % a->kv_heads || (a->d != 64 && a->d != 128) ||
+      a->table_width <= 0 || a->page_size <= 0)
+    return 0;
   const vmo::PagedShape s = vmo::paged_shape(a);
-  return (size_t)((s.waves + (int64_t)a->batch * a->kv_heads * s.blocks) * s.per * (a->d + 2) * 4);
+  return (size_t)((s.waves + (int64_t)a->batch * a->kv_heads * s.blocks) * s.per * (a->d + 2) * 4 + s.waves * 4);
 }
 
 extern "C" int vmo_paged_attention(const vmo_paged_args* a, void* stream) {
@@ -482,7 +515,7 @@ extern "C" int vmo_paged_attention(const vmo_paged_args* a, void* stream) {
     return set_error(VMO_ERR_UNSUPPORTED, "paged_attention: pages of %d tokens (powers of two from 8 to 1024)", a->page_size);
   if (a->batch == 0) return VMO_OK;
   if (a->pages < 1 || a->table_width < 1 || (int64_t)a->table_width * a->page_size > (1ll << 28) ||
-      (int64_t)a->batch * a->heads > (1ll << 30))
+      (int64_t)a->batch * a->heads > (1ll << 30) || a->batch > (1 << 18))   // (sums of 64 sequences wait in 16 KB of LDS)
     return set_error(VMO_ERR_INVALID, "paged_attention: %d pages, %d page numbers a sequence", a->pages, a->table_width);
   if (!a->table || !a->lengths) return set_error(VMO_ERR_INVALID, "paged_attention: no page table or lengths");
   if (!view_ok(a->k) || !view_ok(a->v) || !a->q.data || !a->o.data || !aligned16(a->q.data) || !aligned16(a->o.data) ||
@@ -511,6 +544,7 @@ extern "C" int vmo_paged_attention(const vmo_paged_args* a, void* stream) {
                      (unsigned long long)(a->workspace ? a->workspace_bytes : 0));
   p.part_o = (float*)a->workspace;
   p.part_ml = p.part_o + (p.waves + (int64_t)a->batch * a->kv_heads * p.blocks) * p.per * a->d;
+  p.starts = (int*)(p.part_ml + (p.waves + (int64_t)a->batch * a->kv_heads * p.blocks) * p.per * 2);
   p.c = a->sm_scale * kLog2e;
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = a->dtype == VMO_DTYPE_F16;
