@@ -7,16 +7,20 @@
 //  * a wave's keys fall into three ranges: stages that all its rows see whole (no mask), those on the diagonal (masked),
 //    and those that none sees (skipped; the wave still meets the barriers and copies its share).  Half of the square is
 //    never touched; the diagonal costs a 128-query tile about one stage and a half of its own.
-//  * the reference point m of p = 2^(s c - m) moves only when a lane's block sum leaves [0, 2^15]: then m becomes the row's
-//    maximum and the sums so far are scaled.  p stays below fp16's range, the first block sets m (it starts at -3e38), and
-//    other blocks cost one comparison; a plain running maximum costs 16 more vector operations a block.
+//  * the reference point m of p = 2^(s c - m) moves only when a lane's block sum passes a limit that keeps p within the
+//    16-bit type: then m becomes the row's maximum and the sums so far are scaled.  The first block sets m (it starts at
+//    -3e38).  Even the test for it is left out of the steady loop: its branch behind every block kept the next block's
+//    products waiting (16384 tokens, 12 heads of 128, not causal: 1054 TFLOP/s with it, 1217 without; a running maximum
+//    costs 16 vector operations a block more).  The loop notes that a limit was passed, and then the workgroup runs its
+//    keys again with the test; rows that pass no limit have the same bits both ways.
 //  * workgroups take the heaviest tile first (packed_locate).
 // The row sums add the fp32 p; p is rounded to the 16-bit type as the operand of P V, o once at the end.
 #include "packed.h"
 
 namespace vmo {
 
-constexpr float kSumMost = 32768.f;   // a lane's 16 weights may sum to this before m moves (fp16's P stays finite)
+// a lane's 16 weights of a block may sum to this before m moves: P stays finite in 16 bits (and in bf16 the sums in 32)
+template <bool F16> constexpr float kSumMost = F16 ? 32768.f : 1099511627776.f;
 constexpr float kNoMax = -3.0e38f;    // m of a row that has seen no key
 
 template <int D> constexpr int packed_stage_bytes() { return kFwdBN * D * 2 * 2; }
@@ -82,6 +86,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
 
   const float c = p.c;
   float m_run = kNoMax, l_run = 0.f;
+  bool passed = false;   // some untested block's sum was over the limit
   f32x16 acc[NA];
 #pragma unroll
   for (int a = 0; a < NA; ++a) acc[a] = f32x16{};
@@ -110,8 +115,8 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
     }
   };
   // p = 2^(s c - m) of one block, packed as two B operands, added to the row sum.  nvis: the block's keys below it are
-  // seen (MASKED).
-  auto softmax_block = [&](const f32x16& s, V8 (&P)[2], int nvis, auto masked) __attribute__((always_inline)) {
+  // seen (MASKED); m moves in tested blocks only.
+  auto softmax_block = [&](const f32x16& s, V8 (&P)[2], int nvis, auto masked, auto tested) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked)::value;
     auto seen = [&](int r) __attribute__((always_inline)) { return 8 * (r >> 2) + 4 * hl + (r & 3) < nvis; };
     auto weights = [&]() __attribute__((always_inline)) {
@@ -137,8 +142,10 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
       return ls0 + ls1;
     };
     float ls = weights();
-    const bool over = !(ls <= kSumMost);
-    if (__builtin_amdgcn_ballot_w64(over) != 0) {
+    const bool over = !(ls <= kSumMost<F16>);
+    if constexpr (!decltype(tested)::value) {
+      passed |= over;
+    } else if (__builtin_amdgcn_ballot_w64(over) != 0) {
       // m moves to the row's maximum so far, in the rows that need it (either half of a row's lanes): a row's bits do not
       // depend on its neighbours
       const auto either = __builtin_amdgcn_permlane32_swap(over, over, false, false);
@@ -184,16 +191,16 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
   };
   // a stage that every row of the wave sees whole: S of block 1 beside the softmax of block 0, P V of block 0 beside the
   // softmax of block 1
-  auto full_stage = [&](const VMO_LDS char* Ks) __attribute__((always_inline)) {
+  auto full_stage = [&](const VMO_LDS char* Ks, auto tested) __attribute__((always_inline)) {
     f32x16 s0, s1;
     V8 P0[2], P1[2];
     qk_block(Ks, 0, s0, std::true_type{});
     __builtin_amdgcn_sched_barrier(0);
     qk_block(Ks, 1, s1, std::false_type{});
-    softmax_block(s0, P0, 0, std::false_type{});
+    softmax_block(s0, P0, 0, std::false_type{}, tested);
     __builtin_amdgcn_sched_barrier(0);
     pv_block(Ks + K_BYTES, 0, P0, std::false_type{});
-    softmax_block(s1, P1, 0, std::false_type{});
+    softmax_block(s1, P1, 0, std::false_type{}, tested);
     __builtin_amdgcn_sched_barrier(0);
     pv_block(Ks + K_BYTES, 1, P1, std::true_type{});
   };
@@ -205,7 +212,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
       V8 P[2];
       const int nvis = lim - key0 - 32 * kb2;
       qk_block(Ks, kb2, s, std::false_type{});
-      softmax_block(s, P, nvis, std::true_type{});
+      softmax_block(s, P, nvis, std::true_type{}, std::true_type{});
       masked_product<F16, RB>(acc, Ks + K_BYTES + 32 * kb2 * RB, P, lane, [&](int key) { return key < nvis; });
     }
   };
@@ -213,30 +220,52 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
   // Tile t sits in ring slot t % NSLOT; at its top this wave's copies of it have landed (only those of tile t + 1 may be
   // under way), after the barrier every wave's have, and the slot of tile t - 1 is free for tile t + NSLOT - 1.
   constexpr int kSteadyPending = NSLOT == 3 ? DMA_PER_TILE : 0;
-  if (n_tiles > 0) {
+  const int n_full = live ? uni(min(lo / kFwdBN, n_tiles)) : 0;
+  auto top = [&](int t) __attribute__((always_inline)) {
+    if (NSLOT == 3 && t + 1 < n_tiles) tile_sync<kSteadyPending>();
+    else tile_sync<0>();
+    if (t + NSLOT - 1 < n_tiles) issue(t + NSLOT - 1);
+  };
+  auto slot = [&](int t) __attribute__((always_inline)) { return (const VMO_LDS char*)smem + (t % NSLOT) * STAGE; };
+  for (bool again = false; n_tiles > 0; again = true) {
     issue(0);
     if (NSLOT == 3 && n_tiles > 1) issue(1);
-    const int n_full = live ? uni(min(lo / kFwdBN, n_tiles)) : 0;
-    auto top = [&](int t) __attribute__((always_inline)) {
-      if (NSLOT == 3 && t + 1 < n_tiles) tile_sync<kSteadyPending>();
-      else tile_sync<0>();
-      if (t + NSLOT - 1 < n_tiles) issue(t + NSLOT - 1);
-    };
     int t = 0;
-    for (; t + NSLOT <= n_full; t += NSLOT) {   // slots at compile-time offsets
+    const int tested = again ? n_full : min(1, n_full);   // the first stage sets m
+    for (; t < tested; ++t) {
+      top(t);
+      full_stage(slot(t), std::true_type{});
+    }
+    for (; t + NSLOT <= n_full; t += NSLOT)   // (t = 1, 1 + NSLOT, ..: slots at compile-time offsets)
       static_for<0, NSLOT>([&](auto i) __attribute__((always_inline)) {
         top(t + decltype(i)::value);
-        full_stage((const VMO_LDS char*)smem + decltype(i)::value * STAGE);
+        full_stage((const VMO_LDS char*)smem + ((1 + decltype(i)::value) % NSLOT) * STAGE, std::false_type{});
       });
+    for (; t < n_full; ++t) {
+      top(t);
+      full_stage(slot(t), std::false_type{});
     }
     for (; t < n_tiles; ++t) {
       top(t);
-      const VMO_LDS char* Ks = smem + (t % NSLOT) * STAGE;
-      if (t < n_full) full_stage(Ks);
-      else if (live && t * kFwdBN < hi) masked_stage(Ks, t * kFwdBN);
+      if (live && t * kFwdBN < hi) masked_stage(slot(t), t * kFwdBN);
     }
+    __syncthreads();   // the ring is free
+    if (again) break;
+    // whether any row of the workgroup passed the limit untested: a word a wave in the ring
+    VMO_LDS int* words = (VMO_LDS int*)smem;
+    const bool mine = __builtin_amdgcn_ballot_w64(passed) != 0;
+    if (lane == 0) words[wave] = mine;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < kPackedWaves; ++i) any |= words[i];
+    __syncthreads();
+    if (!any) break;
+    m_run = kNoMax;
+    l_run = 0.f;
+#pragma unroll
+    for (int a = 0; a < NA; ++a) acc[a] = f32x16{};
   }
-  __syncthreads();   // the ring is free: each wave's patch for the row stores
   if (!live) return;
   const float l_tot = wave_sum32(l_run);
   const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;   // (a row that sees no key)
