@@ -10,7 +10,7 @@
 
 namespace vmo {
 
-constexpr int kPackedMaxSeqs = 2048;   // a call's sequences: their tile counts wait in LDS while a workgroup finds its tile
+constexpr int kPackedMaxSeqs = 2048;   // a call's sequences: they wait in LDS while a workgroup finds its tile
 constexpr int kPackedTile = 128;       // queries of a forward / dq workgroup, keys of a dk / dv one
 constexpr int kPackedWaves = 4;
 
@@ -39,6 +39,15 @@ __device__ __forceinline__ int wave_scan_i32(int v) {   // inclusive prefix sum 
   v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
   return v;
+}
+__device__ __forceinline__ int wave_max_i32(int v) {   // of values >= 0
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
 }
 __device__ __forceinline__ int wave_sum_i32(int v) { return __builtin_amdgcn_readlane(wave_scan_i32(v), 63); }
 
@@ -72,41 +81,49 @@ __device__ __forceinline__ int packed_count(const PackedTiles& t, int level) {
 }
 
 struct PackedTile {
-  int seq, tile;   // tile < 0: none; seq then numbers the spare workgroups from 0
-  int spare;       // how many there are
+  PackedSeq s;
+  int tile;           // of the sequence; below 0: none
+  int which, spare;   // then: the spare workgroup's number, and how many there are
 };
+constexpr int kPackedSeqBytes = 16;   // LDS of a sequence while a workgroup finds its tile
 
 // The idx-th tile over all sequences, heaviest first (a tile's time is its keys, or queries: with the heavy ones first the
 // chip's last round is made of light ones).  The largest level that more than idx tiles reach is found by bisection over
-// per-sequence counts that lie in LDS (`lds`: 12 bytes a sequence, free again after the next barrier); a level holds the
-// sequences in order.  Every wave does the same; ~0.3 us for up to 64 sequences.
+// per-sequence counts, from rows and keys that lie in LDS (free again after the call); a level holds the sequences in order.
+// Every wave does the same.
 template <bool KEYS>
 __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int idx, int blocks, VMO_LDS int* lds) {
   const int lane = threadIdx.x & 63;
-  int best = 0;
-  for (int s = threadIdx.x; s < p.n; s += 64 * kPackedWaves) {
-    const PackedTiles t = packed_tiles<KEYS>(p, packed_seq(p, s));
-    lds[3 * s] = t.tiles;
-    lds[3 * s + 1] = t.top;
-    lds[3 * s + 2] = t.cap;
+  for (int s = threadIdx.x; s < p.n; s += (int)blockDim.x) {
+    const PackedSeq q = packed_seq(p, s);
+    *(VMO_LDS i32x4*)(lds + 4 * s) = i32x4{q.qb, q.nq, q.kb, q.nk};
   }
   __syncthreads();
-  auto at = [&](int s) __attribute__((always_inline)) { return PackedTiles{lds[3 * s], lds[3 * s + 1], lds[3 * s + 2]}; };
+  auto seq = [&](int s) __attribute__((always_inline)) {
+    const i32x4 x = *(const VMO_LDS i32x4*)(lds + 4 * s);
+    return PackedSeq{x[0], x[1], x[2], x[3]};
+  };
+  // (up to 64 sequences: one a lane, in registers)
+  const PackedSeq mine = lane < p.n ? seq(lane) : PackedSeq{0, 0, 0, 0};
+  const PackedTiles first = packed_tiles<KEYS>(p, mine);
   auto total = [&](int level) __attribute__((always_inline)) {
-    int c = 0;
-    for (int s = lane; s < p.n; s += 64) c += packed_count(at(s), level);
+    int c = packed_count(first, level);
+    for (int s = lane + 64; s < p.n; s += 64) c += packed_count(packed_tiles<KEYS>(p, seq(s)), level);
     return wave_sum_i32(c);
   };
-  for (int s = lane; s < p.n; s += 64) best = max(best, lds[3 * s] > 0 ? min(lds[3 * s + 1], lds[3 * s + 2]) : 0);
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) best = max(best, __shfl_xor(best, m));
   PackedTile r;
+  r.s = PackedSeq{0, 0, 0, 0};
   const int all = total(0);
   r.spare = blocks - all;
   r.tile = -1;
-  r.seq = idx - all;
+  r.which = idx - all;
   if (idx < all) {
-    int lo = 0, hi = __builtin_amdgcn_readfirstlane(best) + 1;   // total(lo) > idx >= total(hi) = 0
+    int best = first.tiles > 0 ? min(first.top, first.cap) : 0;
+    for (int s = lane + 64; s < p.n; s += 64) {
+      const PackedTiles t = packed_tiles<KEYS>(p, seq(s));
+      best = max(best, t.tiles > 0 ? min(t.top, t.cap) : 0);
+    }
+    int lo = 0, hi = wave_max_i32(best) + 1;   // total(lo) > idx >= total(hi) = 0
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (total(mid) > idx) lo = mid;
@@ -114,22 +131,23 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
     }
     int left = idx - total(lo + 1);
     for (int s0 = 0; s0 < p.n; s0 += 64) {
-      const int s = s0 + lane;
-      const PackedTiles t = s < p.n ? at(s) : PackedTiles{0, 0, 0};
-      const int before = packed_count(t, lo + 1), mine = packed_count(t, lo) - before;
-      const int upto = wave_scan_i32(mine), here = __builtin_amdgcn_readlane(upto, 63);
-      if (left < here) {
+      const PackedSeq q = s0 == 0 ? mine : s0 + lane < p.n ? seq(s0 + lane) : PackedSeq{0, 0, 0, 0};
+      const PackedTiles t = packed_tiles<KEYS>(p, q);
+      const int before = packed_count(t, lo + 1), here = packed_count(t, lo) - before;
+      const int upto = wave_scan_i32(here), sum = __builtin_amdgcn_readlane(upto, 63);
+      if (left < sum) {
         const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > left));
         const int u = __builtin_amdgcn_readlane(before, who) + left -
-                      (__builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(mine, who));
-        r.seq = s0 + who;
+                      (__builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(here, who));
+        r.s = PackedSeq{__builtin_amdgcn_readlane(q.qb, who), __builtin_amdgcn_readlane(q.nq, who),
+                        __builtin_amdgcn_readlane(q.kb, who), __builtin_amdgcn_readlane(q.nk, who)};
         r.tile = KEYS || !p.causal ? u : __builtin_amdgcn_readlane(t.tiles, who) - 1 - u;
         break;
       }
-      left -= here;
+      left -= sum;
     }
   }
-  __syncthreads();   // every wave has read the counts
+  __syncthreads();   // every wave has read the sequences
   return r;
 }
 
@@ -142,7 +160,7 @@ __device__ __forceinline__ void packed_zero_rest(T* rows, int64_t sn, const int3
   constexpr int CH = D / 8;
   const int first = min(max(off[0], 0), total), last = min(max(off[n], 0), total);
   for (int r0 = which * kPackedTile; r0 < total; r0 += spare * kPackedTile)
-    for (int i = threadIdx.x; i < kPackedTile * CH; i += 64 * kPackedWaves) {
+    for (int i = threadIdx.x; i < kPackedTile * CH; i += (int)blockDim.x) {
       const int r = r0 + i / CH;
       if (r < total && (r < first || r >= last)) *(uint4*)((char*)(rows + r * sn) + (i % CH) * 16) = uint4{0, 0, 0, 0};
     }
@@ -154,8 +172,9 @@ template <bool F16> constexpr uint32_t kInfBits = F16 ? 0x7c00u : 0x7f80u;   // 
 // acc[a] += W^T P for 32 rows W of an LDS tile (RB-byte rows, swizzled) and the packed weights P of the accumulator layout
 // (element e of P[h]: row 16 h + 8 (e / 4) + 4 hl + e % 4 of the lane's column).  Rows that the lane's column does not see
 // have weight 0, but 0 times an infinity or NaN is a NaN: where a wave's operands hold such values they are taken as 0,
-// and a second pass adds them to the columns that do see their row.
-template <bool F16, int RB, int NA, class Sees>
+// and a second pass adds them to the columns that do see their row.  STEP accumulator blocks are tested at a time: all of
+// them where the registers hold their operands (one branch), else one.
+template <bool F16, int RB, int STEP, int NA, class Sees>
 __device__ __forceinline__ void masked_product(f32x16 (&acc)[NA], const VMO_LDS char* W, const typename Elem<F16>::V8 (&P)[2],
                                                int lane, Sees sees) {
   using E = Elem<F16>;
@@ -170,30 +189,33 @@ __device__ __forceinline__ void masked_product(f32x16 (&acc)[NA], const VMO_LDS 
   const int trow = 4 * hl + ((lane & 15) >> 2), tchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), tbyte = (lane & 1) * 8;
   bool odd = false;
 #pragma unroll
-  for (int a = 0; a < NA; ++a) {
-    V8 w[2];
+  for (int a0 = 0; a0 < NA; a0 += STEP) {
+    V8 w[2 * STEP];
     u16x2 big = {0, 0};
-    const int c0 = trow * RB + (((4 * a + tchunk) ^ swz_rows<RB>(trow)) * 16 + tbyte);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const VMO_LDS char* rp = W + 16 * h * RB;
-      w[h] = lds_read_tr8<V8>(rp + c0, rp + 8 * RB + (c0 ^ 32));
-      const u32x4 bits = __builtin_bit_cast(u32x4, w[h]);
+    for (int i = 0; i < 2 * STEP; ++i) {
+      const int c0 = trow * RB + (((4 * (a0 + i / 2) + tchunk) ^ swz_rows<RB>(trow)) * 16 + tbyte);
+      const VMO_LDS char* rp = W + 16 * (i % 2) * RB;
+      w[i] = lds_read_tr8<V8>(rp + c0, rp + 8 * RB + (c0 ^ 32));
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * STEP; ++i) {
+      const u32x4 bits = __builtin_bit_cast(u32x4, w[i]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, bits[j] & 0x7fff7fffu));
     }
     if (__builtin_amdgcn_ballot_w64(max((uint32_t)big[0], (uint32_t)big[1]) >= kInfBits<F16>) != 0) {
       odd = true;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u16x8 b = __builtin_bit_cast(u16x8, w[h]);
+      for (int i = 0; i < 2 * STEP; ++i) {
+        u16x8 b = __builtin_bit_cast(u16x8, w[i]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) b[e] = (b[e] & 0x7fff) >= kInfBits<F16> ? 0 : b[e];
-        w[h] = __builtin_bit_cast(V8, b);
+        w[i] = __builtin_bit_cast(V8, b);
       }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) acc[a] = E::mfma(w[h], P[h], acc[a]);
+    for (int i = 0; i < 2 * STEP; ++i) acc[a0 + i / 2] = E::mfma(w[i], P[i % 2], acc[a0 + i / 2]);
   }
   if (odd) {
 #pragma unroll 1

@@ -19,7 +19,7 @@ constexpr int kKvQueries = 32;   // queries of a dk / dv stage
 
 template <int D> constexpr int packed_dq_lds() {
   constexpr int ring = 2 * kDqKeys * D * 2 * 2;
-  constexpr int least = kPackedWaves * kEpiPatchBytes > 12 * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : 12 * kPackedMaxSeqs;
+  constexpr int least = kPackedWaves * kEpiPatchBytes > kPackedSeqBytes * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : kPackedSeqBytes * kPackedMaxSeqs;
   return ring > least ? ring : least;
 }
 // V's 128 rows in LDS at D = 128 (in registers they would spill)
@@ -27,7 +27,7 @@ template <int D> constexpr bool packed_v_in_lds() { return D >= 128; }
 template <int D> constexpr int packed_kv_stage() { return kKvQueries * D * 2 * 2 + 512; }
 template <int D> constexpr int packed_kv_lds() {
   constexpr int ring = 2 * packed_kv_stage<D>() + (packed_v_in_lds<D>() ? kPackedTile * D * 2 : 0);
-  constexpr int least = kPackedWaves * kEpiPatchBytes > 12 * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : 12 * kPackedMaxSeqs;
+  constexpr int least = kPackedWaves * kEpiPatchBytes > kPackedSeqBytes * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : kPackedSeqBytes * kPackedMaxSeqs;
   return ring > least ? ring : least;
 }
 
@@ -52,11 +52,10 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
   const int head = uni(packed_head((int)blockIdx.x % p.heads, p.heads));
   const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, (VMO_LDS int*)smem);
   if (w.tile < 0) {
-    packed_zero_rest<T, D>((T*)p.dq + head * p.dq_sh, p.dq_sn, p.q_off, p.n, p.tq, w.seq, w.spare);
+    packed_zero_rest<T, D>((T*)p.dq + head * p.dq_sh, p.dq_sn, p.q_off, p.n, p.tq, w.which, w.spare);
     return;
   }
-  const PackedSeq sq = packed_seq(p, uni(w.seq));
-  const int nq = uni(sq.nq), nk = uni(sq.nk), qb = uni(sq.qb), kb = uni(sq.kb);
+  const int nq = uni(w.s.nq), nk = uni(w.s.nk), qb = uni(w.s.qb), kb = uni(w.s.kb);
   const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int q0 = uni(w.tile) * kPackedTile + wave * 32;
   const bool live = q0 < nq;
@@ -146,7 +145,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
 #pragma unroll
       for (int kb2 = 0; kb2 < 2; ++kb2) {
         const int nvis = lim - t * kDqKeys - 32 * kb2;
-        masked_product<F16, RB>(acc, Ks + 32 * kb2 * RB, G[kb2], lane, [&](int key) { return key < nvis; });
+        masked_product<F16, RB, 1>(acc, Ks + 32 * kb2 * RB, G[kb2], lane, [&](int key) { return key < nvis; });
       }
     } else {
       prefetched_chain<4 * NA, PF>(
@@ -201,13 +200,12 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   const PackedTile w = packed_locate<true>(p, (int)blockIdx.x / shares, (int)gridDim.x / shares, (VMO_LDS int*)smem);
   if (w.tile < 0) {
     if (p.splits == 1) {
-      packed_zero_rest<T, D>((T*)p.dk + kvh * p.dk_sh, p.dk_sn, p.k_off, p.n, p.tk, w.seq, w.spare);
-      packed_zero_rest<T, D>((T*)p.dv + kvh * p.dv_sh, p.dv_sn, p.k_off, p.n, p.tk, w.seq, w.spare);
+      packed_zero_rest<T, D>((T*)p.dk + kvh * p.dk_sh, p.dk_sn, p.k_off, p.n, p.tk, w.which, w.spare);
+      packed_zero_rest<T, D>((T*)p.dv + kvh * p.dv_sh, p.dv_sn, p.k_off, p.n, p.tk, w.which, w.spare);
     }
     return;
   }
-  const PackedSeq sq = packed_seq(p, uni(w.seq));
-  const int nq = uni(sq.nq), nk = uni(sq.nk), qb = uni(sq.qb), kb = uni(sq.kb);
+  const int nq = uni(w.s.nq), nk = uni(w.s.nk), qb = uni(w.s.qb), kb = uni(w.s.kb);
   const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int tile0 = uni(w.tile) * kPackedTile, k0 = tile0 + wave * 32;
   const bool live = k0 < nk;
@@ -324,8 +322,8 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
       }
     }
     if constexpr (MASKED) {
-      masked_product<F16, RB>(dv, dOs, P, lane, sees);
-      masked_product<F16, RB>(dk, Qs, G, lane, sees);
+      masked_product<F16, RB, 1>(dv, dOs, P, lane, sees);
+      masked_product<F16, RB, 1>(dk, Qs, G, lane, sees);
     } else {
       prefetched_chain<4 * NA, PF>(
           [&](int i) __attribute__((always_inline)) {

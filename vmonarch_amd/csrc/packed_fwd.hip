@@ -14,6 +14,8 @@
 //    costs 16 vector operations a block more).  The loop notes that a limit was passed, and then the workgroup runs its
 //    keys again with the test; rows that pass no limit have the same bits both ways.
 //  * workgroups take the heaviest tile first (packed_locate).
+//  * where the launch is small, eight waves share the 128 queries: two groups of four take every other stage, each with a
+//    ring of its own, and the second's sums join the first's in LDS (G = 2).
 // The row sums add the fp32 p; p is rounded to the 16-bit type as the operand of P V, o once at the end.
 #include "packed.h"
 
@@ -24,14 +26,14 @@ template <bool F16> constexpr float kSumMost = F16 ? 32768.f : 1099511627776.f;
 constexpr float kNoMax = -3.0e38f;    // m of a row that has seen no key
 
 template <int D> constexpr int packed_stage_bytes() { return kFwdBN * D * 2 * 2; }
-template <int D> constexpr int packed_fwd_lds() {
-  constexpr int ring = fwd_slots(packed_stage_bytes<D>()) * packed_stage_bytes<D>();
-  constexpr int least = kPackedWaves * kEpiPatchBytes > 12 * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : 12 * kPackedMaxSeqs;
+template <int D, int G> constexpr int packed_fwd_lds() {
+  constexpr int ring = G * fwd_slots(packed_stage_bytes<D>()) * packed_stage_bytes<D>();
+  constexpr int least = kPackedWaves * kEpiPatchBytes > kPackedSeqBytes * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : kPackedSeqBytes * kPackedMaxSeqs;
   return ring > least ? ring : least;
 }
 
-template <bool F16, int D>
-__global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(PackedParams p) {
+template <bool F16, int D, int G>
+__global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kernel(PackedParams p) {
   using E = Elem<F16>;
   using T = typename E::T;
   using V8 = typename E::V8;
@@ -41,19 +43,20 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
   constexpr int DMA_PER_TILE = STAGE / 1024 / kPackedWaves;
   extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
   VMO_LDS char* smem = (VMO_LDS char*)smem_raw;
-  const uint32_t smem_u32 = (uint32_t)(uintptr_t)smem;
   auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
 
   const int head = uni(packed_head((int)blockIdx.x % p.heads, p.heads));
   const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, (VMO_LDS int*)smem);
   if (w.tile < 0) {
     if (p.zero_rest)
-      packed_zero_rest<T, D>((T*)p.out + head * p.o_sh, p.o_sn, p.q_off, p.n, p.tq, w.seq, w.spare);
+      packed_zero_rest<T, D>((T*)p.out + head * p.o_sh, p.o_sn, p.q_off, p.n, p.tq, w.which, w.spare);
     return;
   }
-  const PackedSeq sq = packed_seq(p, uni(w.seq));
-  const int nq = uni(sq.nq), nk = uni(sq.nk), qb = uni(sq.qb), kb = uni(sq.kb);
-  const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
+  const int nq = uni(w.s.nq), nk = uni(w.s.nk), qb = uni(w.s.qb), kb = uni(w.s.kb);
+  const int tid = threadIdx.x, wave = uni((tid >> 6) % kPackedWaves), grp = G > 1 ? uni((tid >> 6) / kPackedWaves) : 0;
+  const int lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
+  VMO_LDS char* ring = smem + grp * NSLOT * STAGE;   // the key group's own
+  const uint32_t ring_u32 = (uint32_t)(uintptr_t)ring;
   const int q0 = uni(w.tile) * kPackedTile + wave * 32;   // the wave's first row of the sequence
   const bool live = q0 < nq;
   // keys that row i sees: the first sees(i) of the sequence
@@ -62,10 +65,26 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
   const int row = min(q0 + l32, nq - 1);
   const int lim = keys_of(row);
   const int lo = uni(keys_of(min(q0, nq - 1))), hi = uni(keys_of(min(q0 + 31, nq - 1)));   // least and most of the wave
-  const int n_tiles = uni((keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 1, nq - 1)) + kFwdBN - 1) / kFwdBN);
+  const int all_tiles = uni((keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 1, nq - 1)) + kFwdBN - 1) / kFwdBN);
+
+  const int n_tiles = G > 1 ? (all_tiles - grp + G - 1) / G : all_tiles, steps = (all_tiles + G - 1) / G;   // the group's tiles
 
   const T* kbase = (const T*)p.k + (int64_t)(head / p.group) * p.k_sh + (int64_t)kb * p.k_sn;
   const T* vbase = (const T*)p.v + (int64_t)(head / p.group) * p.v_sh + (int64_t)kb * p.v_sn;
+  const TileCopy<T, D, kPackedWaves> kcopy(kbase, p.k_sn, wave, lane), vcopy(vbase, p.v_sn, wave, lane);
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    uint32_t sb = ring_u32;
+    asm volatile("" : "+s"(sb));
+    const uint32_t st = sb + (uint32_t)((t % NSLOT) * STAGE);
+    kcopy.issue((t * G + grp) * kFwdBN, nk, st);   // (a tile that runs past the sequence repeats its last key: masked)
+    vcopy.issue((t * G + grp) * kFwdBN, nk, st + K_BYTES);
+  };
+
+  auto prime = [&]() __attribute__((always_inline)) {
+    if (n_tiles > 0) issue(0);
+    if (NSLOT == 3 && n_tiles > 1) issue(1);
+  };
+  prime();   // the first copies are under way while the queries come
   V8 qf[NDS];   // Q^T as the B operand: lane (query l32, half hl) holds features 16 ds + 8 hl + 0..7
   {
     const T* qp = (const T*)p.q + (int64_t)head * p.q_sh + (int64_t)(qb + row) * p.q_sn + hl * 8;
@@ -75,14 +94,6 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
       asm volatile("" : "+v"(qf[ds]));
     }
   }
-  const TileCopy<T, D, kPackedWaves> kcopy(kbase, p.k_sn, wave, lane), vcopy(vbase, p.v_sn, wave, lane);
-  auto issue = [&](int t) __attribute__((always_inline)) {
-    uint32_t sb = smem_u32;
-    asm volatile("" : "+s"(sb));
-    const uint32_t st = sb + (uint32_t)((t % NSLOT) * STAGE);
-    kcopy.issue(t * kFwdBN, nk, st);   // (a tile that runs past the sequence repeats its last key: masked)
-    vcopy.issue(t * kFwdBN, nk, st + K_BYTES);
-  };
 
   const float c = p.c;
   float m_run = kNoMax, l_run = 0.f;
@@ -204,32 +215,36 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
     __builtin_amdgcn_sched_barrier(0);
     pv_block(Ks + K_BYTES, 1, P1, std::true_type{});
   };
+  // a stage on the diagonal, or at the end: both blocks' S first
   auto masked_stage = [&](const VMO_LDS char* Ks, int key0) __attribute__((always_inline)) {
-#pragma unroll 1
+    f32x16 s[2];
+    const bool two = key0 + 32 < hi;
+    qk_block(Ks, 0, s[0], std::false_type{});
+    if (two) qk_block(Ks, 1, s[1], std::false_type{});
+#pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
-      if (key0 + 32 * kb2 >= hi) break;
-      f32x16 s;
+      if (kb2 == 1 && !two) break;
       V8 P[2];
       const int nvis = lim - key0 - 32 * kb2;
-      qk_block(Ks, kb2, s, std::false_type{});
-      softmax_block(s, P, nvis, std::true_type{}, std::true_type{});
-      masked_product<F16, RB>(acc, Ks + K_BYTES + 32 * kb2 * RB, P, lane, [&](int key) { return key < nvis; });
+      softmax_block(s[kb2], P, nvis, std::true_type{}, std::true_type{});
+      masked_product<F16, RB, NA>(acc, Ks + K_BYTES + 32 * kb2 * RB, P, lane, [&](int key) { return key < nvis; });
     }
   };
 
   // Tile t sits in ring slot t % NSLOT; at its top this wave's copies of it have landed (only those of tile t + 1 may be
   // under way), after the barrier every wave's have, and the slot of tile t - 1 is free for tile t + NSLOT - 1.
   constexpr int kSteadyPending = NSLOT == 3 ? DMA_PER_TILE : 0;
-  const int n_full = live ? uni(min(lo / kFwdBN, n_tiles)) : 0;
+  const int n_full = live ? uni(min((lo / kFwdBN - grp + G - 1) / G, n_tiles)) : 0;
   auto top = [&](int t) __attribute__((always_inline)) {
     if (NSLOT == 3 && t + 1 < n_tiles) tile_sync<kSteadyPending>();
     else tile_sync<0>();
     if (t + NSLOT - 1 < n_tiles) issue(t + NSLOT - 1);
   };
-  auto slot = [&](int t) __attribute__((always_inline)) { return (const VMO_LDS char*)smem + (t % NSLOT) * STAGE; };
-  for (bool again = false; n_tiles > 0; again = true) {
-    issue(0);
-    if (NSLOT == 3 && n_tiles > 1) issue(1);
+  auto slot = [&](int t) __attribute__((always_inline)) { return (const VMO_LDS char*)ring + (t % NSLOT) * STAGE; };
+  // stages that some wave of the workgroup runs untested (the last wave's rows see most)
+  const int untested = uni(max(keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 32, nq - 1)) / kFwdBN - G, 0));
+  for (bool again = false; steps > 0; again = true) {
+    if (again) prime();
     int t = 0;
     const int tested = again ? n_full : min(1, n_full);   // the first stage sets m
     for (; t < tested; ++t) {
@@ -239,26 +254,27 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
     for (; t + NSLOT <= n_full; t += NSLOT)   // (t = 1, 1 + NSLOT, ..: slots at compile-time offsets)
       static_for<0, NSLOT>([&](auto i) __attribute__((always_inline)) {
         top(t + decltype(i)::value);
-        full_stage((const VMO_LDS char*)smem + ((1 + decltype(i)::value) % NSLOT) * STAGE, std::false_type{});
+        full_stage((const VMO_LDS char*)ring + ((1 + decltype(i)::value) % NSLOT) * STAGE, std::false_type{});
       });
     for (; t < n_full; ++t) {
       top(t);
       full_stage(slot(t), std::false_type{});
     }
-    for (; t < n_tiles; ++t) {
+    for (; t < steps; ++t) {
       top(t);
-      if (live && t * kFwdBN < hi) masked_stage(slot(t), t * kFwdBN);
+      const int key0 = (t * G + grp) * kFwdBN;
+      if (live && key0 < hi) masked_stage(slot(t), key0);
     }
     __syncthreads();   // the ring is free
-    if (again) break;
+    if (again || untested == 0) break;
     // whether any row of the workgroup passed the limit untested: a word a wave in the ring
     VMO_LDS int* words = (VMO_LDS int*)smem;
     const bool mine = __builtin_amdgcn_ballot_w64(passed) != 0;
-    if (lane == 0) words[wave] = mine;
+    if (lane == 0) words[grp * kPackedWaves + wave] = mine;
     __syncthreads();
     int any = 0;
 #pragma unroll
-    for (int i = 0; i < kPackedWaves; ++i) any |= words[i];
+    for (int i = 0; i < G * kPackedWaves; ++i) any |= words[i];
     __syncthreads();
     if (!any) break;
     m_run = kNoMax;
@@ -266,29 +282,64 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
 #pragma unroll
     for (int a = 0; a < NA; ++a) acc[a] = f32x16{};
   }
+  float l_tot = wave_sum32(l_run);
+  if constexpr (G > 1) {   // the second group's sums join the first's, through LDS (a lane reads what its fellow wrote)
+    static_assert(G == 2 && kPackedWaves * (NA * 16 + 2) * 256 <= G * NSLOT * STAGE, "two groups");
+    VMO_LDS float* box = (VMO_LDS float*)(smem + wave * (NA * 16 + 2) * 256) + lane;
+    if (grp == 1) {
+      box[0] = m_run;
+      box[64] = l_tot;
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) box[(2 + a * 16 + r) * 64] = acc[a][r];
+    }
+    __syncthreads();
+    if (grp == 1) return;
+    const float m1 = box[0], m = fmaxf(m_run, m1), f0 = fast_exp2(m_run - m), f1 = fast_exp2(m1 - m);
+    l_tot = fmaf(l_tot, f0, box[64] * f1);
+    m_run = m;
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][r] = fmaf(acc[a][r], f0, box[(2 + a * 16 + r) * 64] * f1);
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    // (each wave's row patch lies in its own box)
+  }
   if (!live) return;
-  const float l_tot = wave_sum32(l_run);
   const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;   // (a row that sees no key)
   const int nrows = min(32, nq - q0);
   T* out = (T*)p.out + (int64_t)head * p.o_sh + (int64_t)(qb + q0) * p.o_sn;
-  store_acc_rows<F16>((VMO_LDS float*)(smem + wave * kEpiPatchBytes), acc, NA, inv, kGradStore, (char*)out, p.o_sn * 2, nrows,
+  store_acc_rows<F16>((VMO_LDS float*)(smem + wave * (G > 1 ? (NA * 16 + 2) * 256 : kEpiPatchBytes)), acc, NA, inv, kGradStore, (char*)out, p.o_sn * 2, nrows,
                       lane);
   if (p.lse && hl == 0 && l32 < nrows)
     p.lse[(int64_t)head * p.st_sh + qb + q0 + l32] = l_tot == 0.f ? 0.f : m_run + fast_log2(l_tot);
 }
 
-template <bool F16, int D>
-static int launch_packed_fwd(const PackedParams& p, hipStream_t s) {
-  constexpr int LDS = packed_fwd_lds<D>();
-  static_assert(LDS <= 65536, "LDS within the default limit");
-  const int64_t grid = ((int64_t)(p.tq + kPackedTile - 1) / kPackedTile + p.n) * p.heads;
-  hipLaunchKernelGGL((packed_fwd_kernel<F16, D>), dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS, s, p);
+template <bool F16, int D, int G>
+static int launch_packed_fwd(const PackedParams& p, int64_t grid, hipStream_t s) {
+  constexpr int LDS = packed_fwd_lds<D, G>();
+  auto kern = packed_fwd_kernel<F16, D, G>;
+  if (LDS > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
+    return set_error(VMO_ERR_LAUNCH, "packed_fwd: cannot raise the LDS limit to %d bytes", LDS);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kPackedWaves * G), LDS, s, p);
   return launch_status("packed_fwd");
 }
 
+template <bool F16, int D>
+static int dispatch_packed_fwd(const PackedParams& p, hipStream_t s) {
+  const int64_t grid = ((int64_t)(p.tq + kPackedTile - 1) / kPackedTile + p.n) * p.heads;
+  // Two key groups halve the longest workgroup's time, which is the launch's where the chip holds all of them at once (one
+  // prompt of 4096 tokens, 12 heads of 128: 80.2 -> 65.7 us, of 2048: 38.8 -> 34.7); with more workgroups, the barriers
+  // that eight waves share cost (8192 tokens 214.6 -> 224.4 us), and for short prompts the join does (four of up to 200
+  // tokens, 64 wide: 8.9 -> 9.6 us).
+  const bool two = grid <= 512 && p.tk >= 768ll * p.n;
+  return two ? launch_packed_fwd<F16, D, 2>(p, grid, s) : launch_packed_fwd<F16, D, 1>(p, grid, s);
+}
+
 int packed_fwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s) {
-  if (d == 64) return f16 ? launch_packed_fwd<true, 64>(p, s) : launch_packed_fwd<false, 64>(p, s);
-  return f16 ? launch_packed_fwd<true, 128>(p, s) : launch_packed_fwd<false, 128>(p, s);
+  if (d == 64) return f16 ? dispatch_packed_fwd<true, 64>(p, s) : dispatch_packed_fwd<false, 64>(p, s);
+  return f16 ? dispatch_packed_fwd<true, 128>(p, s) : dispatch_packed_fwd<false, 128>(p, s);
 }
 
 }  // namespace vmo
