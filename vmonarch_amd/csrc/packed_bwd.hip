@@ -250,9 +250,11 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
     const int row0 = t_next * kKvQueries;
     qcopy.issue(row0, nq, st);
     docopy.issue(row0, nq, st + Q_BYTES);
-    if (wave == 0) {   // lanes 0-31: lse, 32-63: -delta
-      const int qi = min(row0 + l32, nq - 1);
-      dma4_async(hl ? nd_h + qi : lse_h + qi, st + 2 * Q_BYTES);
+    if (wave == 0) {   // the rows' lse and -delta (64 places each, 32 used), from scalar bases: as 64-bit lane addresses they
+      // were kept in scratch, whose reload waits for every copy in flight
+      const uint32_t at = (uint32_t)min(row0 + lane, nq - 1) * 4;
+      dma4_async_s((uint64_t)(uintptr_t)lse_h, at, st + 2 * Q_BYTES);
+      dma4_async_s((uint64_t)(uintptr_t)nd_h, at, st + 2 * Q_BYTES + 256);
     }
     if (++t_next == t1) {
       t_next = t0;
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
     f32x16 s = f32x16{}, dp;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {   // dP starts from -delta
-      const f32x4 av = *(const VMO_LDS f32x4*)(sts + 32 + 8 * g + 4 * hl);
+      const f32x4 av = *(const VMO_LDS f32x4*)(sts + 64 + 8 * g + 4 * hl);
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * g + e] = av[e];
     }

@@ -143,6 +143,13 @@ __device__ __forceinline__ void dma16_async_s(uint64_t sbase, uint32_t voff, uin
                : "v"(voff), "s"(uniform64(sbase)), "s"(__builtin_amdgcn_readfirstlane(lds_wave_base))
                : "m0");
 }
+// As dma4_async, from a scalar base and per-lane byte offsets.
+__device__ __forceinline__ void dma4_async_s(uint64_t sbase, uint32_t voff, uint32_t lds_wave_base) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1"
+               :
+               : "v"(voff), "s"(uniform64(sbase)), "s"(__builtin_amdgcn_readfirstlane(lds_wave_base))
+               : "m0");
+}
 #pragma clang diagnostic pop
 
 // Workgroup barrier for a dma16_async pipeline: this wave's own copies except the newest
