@@ -341,12 +341,12 @@ typedef struct vmo_packed_args {
   float* lse;
   int64_t stat_stride;
   float sm_scale;
-  /* backward only */
-  vmo_view grad_o, grad_q, grad_k, grad_v;
+  vmo_view grad_o, grad_q, grad_k, grad_v; /* backward only */
   void* workspace;
   size_t workspace_bytes;
 } vmo_packed_args;
 
+size_t vmo_packed_fwd_workspace_size(const vmo_packed_args* args);
 int vmo_packed_fwd(const vmo_packed_args* args, void* stream);
 size_t vmo_packed_bwd_workspace_size(const vmo_packed_args* args);
 int vmo_packed_bwd(const vmo_packed_args* args, void* stream);

@@ -145,9 +145,9 @@ def lib():
         L.vmo_fea_bwd_workspace_size.argtypes = [ctypes.POINTER(FeaBwdArgs)]
         L.vmo_fea_bwd.restype = ctypes.c_int
         L.vmo_fea_bwd.argtypes = [ctypes.POINTER(FeaBwdArgs), c_void_p]
-        L.vmo_packed_bwd_workspace_size.restype = L.vmo_paged_attention_workspace_size.restype = c_size_t
-        L.vmo_packed_bwd_workspace_size.argtypes = [ctypes.POINTER(PackedArgs)]
-        L.vmo_paged_attention_workspace_size.argtypes = [ctypes.POINTER(PagedArgs)]
+        for name, args in (("vmo_packed_fwd", PackedArgs), ("vmo_packed_bwd", PackedArgs), ("vmo_paged_attention", PagedArgs)):
+            f = getattr(L, name + "_workspace_size")
+            f.restype, f.argtypes = c_size_t, [ctypes.POINTER(args)]
         for name, args in (("vmo_packed_fwd", PackedArgs), ("vmo_packed_bwd", PackedArgs), ("vmo_paged_attention", PagedArgs),
                            ("vmo_append_pages", AppendArgs), ("vmo_copy_pages", CopyArgs)):
             f = getattr(L, name)

@@ -657,6 +657,12 @@ std::tuple<Tensor, OptT> packed_fwd(const Tensor& q_in, const Tensor& k_in, cons
   }
   a.o = rows_view(o);
   a.zero_rest = !out;
+  Tensor ws;
+  if (const size_t bytes = vmo_packed_fwd_workspace_size(&a)) {
+    ws = workspace(bytes, q);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = bytes;
+  }
   check(vmo_packed_fwd(&a, stream_of(q)), "vmo_packed_fwd");
   return {o, lse};
 }

@@ -25,8 +25,10 @@ struct PackedParams {
   float* lse;                              // (heads, tq), log2 units, rows of st_sh
   int64_t st_sh;
   float* neg_delta;                        // (heads, tq): -rowsum(o dO), from the dq kernel to the dk / dv one
-  float *dk_part, *dv_part;                // (splits, kv_heads, tk, D) fp32 when the group's heads are split
-  int splits;                              // workgroups that share a key tile, each with group / splits of the heads
+  float *part, *part2;                     // parts of split tiles: (slots, 128, D) fp32 sums; the forward's m and l (.., 2), or dv's
+                                           // (splits > 1: dk's and dv's (splits, kv_heads, tk, D))
+  int splits;                              // dk / dv: workgroups that share a key tile, each with group / splits of the heads
+  int split_least;                         // tiles of up to so many units are never split (0: no tile is)
   float c, sm_scale;                       // c = sm_scale log2 e
 };
 
@@ -80,19 +82,56 @@ __device__ __forceinline__ int packed_count(const PackedTiles& t, int level) {
   return level <= t.cap ? min(max(t.top - level + 1, 0), t.tiles) : 0;
 }
 
+// Heavy tiles are split: one long prompt's last tile sees all its keys, and alone took longer than the average workgroup slot
+// has work (8 heads of 128, prompts of 12000 and 4384 tokens: 188 stages of a mean of 78, and the CUs idle 29 % of the
+// forward; split, it takes 336 us instead of 372, dq 470 instead of 500).  A tile of more than S units is cut into
+// ceil(L / S) parts of equal length, S the mean work of the chip's kPackedSlots workgroups (smaller parts balance no better:
+// their sums' traffic grows; 336 -> 357 us with half of S) and `split_least` at least.  All parts together are at most two
+// for every slot, they come first in the order, and their fp32 sums go to slot = workgroup number; a second kernel adds them
+// in order.
+constexpr int kPackedSlots = 512;
+constexpr int kPackedParts = 2 * kPackedSlots;
+struct PackedSplit {
+  int S;
+  __device__ __forceinline__ int parts(int L) const { return L > S ? (L + S - 1) / S : 1; }
+  // parts of one tile each of the levels 1 .. x
+  __device__ __forceinline__ int upto(int x) const {
+    if (x <= S) return max(x, 0);
+    const int q = x / S, r = x - q * S;
+    return S * (q * (q + 1) / 2) + r * (q + 1);
+  }
+  // parts of a sequence's tiles of at least the work `level`
+  __device__ __forceinline__ int count(const PackedTiles& t, int level) const {
+    const int n_cap = min(max(t.top - t.cap + 1, 0), t.tiles);   // tiles of work `cap`; the others' falls by one
+    const int from = max(level, max(t.top - t.tiles + 1, 1)), most = min(t.cap - 1, t.top);
+    int c = max(level, 1) <= t.cap ? n_cap * parts(t.cap) : 0;
+    if (most >= from) c += upto(most) - upto(from - 1);
+    if (level <= 0) c += t.tiles - packed_count(t, 1);   // tiles without work
+    return c;
+  }
+};
+// the work of a sequence's tiles
+__device__ __forceinline__ float packed_work(const PackedTiles& t) {
+  const int n_cap = min(max(t.top - t.cap + 1, 0), t.tiles);
+  const int most = min(t.cap - 1, t.top), least = max(t.top - t.tiles + 1, 1);
+  const float m = (float)most, l = (float)least;
+  return (float)n_cap * (float)t.cap + (most >= least ? 0.5f * (m + l) * (m - l + 1.f) : 0.f);
+}
+
 struct PackedTile {
   PackedSeq s;
   int tile;           // of the sequence; below 0: none
-  int which, spare;   // then: the spare workgroup's number, and how many there are
+  int part, parts;
+  int which, spare;   // of no tile: the spare workgroup's number, and how many there are
 };
 constexpr int kPackedSeqBytes = 16;   // LDS of a sequence while a workgroup finds its tile
 
-// The idx-th tile over all sequences, heaviest first (a tile's time is its keys, or queries: with the heavy ones first the
-// chip's last round is made of light ones).  The largest level that more than idx tiles reach is found by bisection over
-// per-sequence counts, from rows and keys that lie in LDS (free again after the call); a level holds the sequences in order.
-// Every wave does the same.
+// The idx-th part over all sequences' tiles, heaviest tiles first (a tile's time is its keys, or queries: with the heavy ones
+// first the chip's last round is made of light ones); `heads` workgroups take each.  The largest level whose parts and those
+// above are more than idx is found by bisection over per-sequence counts, from rows and keys that lie in LDS (free again
+// after the call); a level holds the sequences in order.  Every wave does the same.
 template <bool KEYS>
-__device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int idx, int blocks, VMO_LDS int* lds) {
+__device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int idx, int blocks, int heads, VMO_LDS int* lds) {
   const int lane = threadIdx.x & 63;
   for (int s = threadIdx.x; s < p.n; s += (int)blockDim.x) {
     const PackedSeq q = packed_seq(p, s);
@@ -106,9 +145,17 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
   // (up to 64 sequences: one a lane, in registers)
   const PackedSeq mine = lane < p.n ? seq(lane) : PackedSeq{0, 0, 0, 0};
   const PackedTiles first = packed_tiles<KEYS>(p, mine);
+  PackedSplit split{1 << 28};
+  if (p.split_least > 0) {
+    float work = packed_work(first);
+    for (int s = lane + 64; s < p.n; s += 64) work += packed_work(packed_tiles<KEYS>(p, seq(s)));
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) work += __shfl_xor(work, m);
+    split.S = max(__builtin_amdgcn_readfirstlane((int)ceilf(work * (float)heads * (1.001f / kPackedSlots))), p.split_least);
+  }
   auto total = [&](int level) __attribute__((always_inline)) {
-    int c = packed_count(first, level);
-    for (int s = lane + 64; s < p.n; s += 64) c += packed_count(packed_tiles<KEYS>(p, seq(s)), level);
+    int c = split.count(first, level);
+    for (int s = lane + 64; s < p.n; s += 64) c += split.count(packed_tiles<KEYS>(p, seq(s)), level);
     return wave_sum_i32(c);
   };
   PackedTile r;
@@ -116,6 +163,8 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
   const int all = total(0);
   r.spare = blocks - all;
   r.tile = -1;
+  r.part = 0;
+  r.parts = 1;
   r.which = idx - all;
   if (idx < all) {
     int best = first.tiles > 0 ? min(first.top, first.cap) : 0;
@@ -130,18 +179,21 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
       else hi = mid;
     }
     int left = idx - total(lo + 1);
+    const int P = split.parts(lo);
     for (int s0 = 0; s0 < p.n; s0 += 64) {
       const PackedSeq q = s0 == 0 ? mine : s0 + lane < p.n ? seq(s0 + lane) : PackedSeq{0, 0, 0, 0};
       const PackedTiles t = packed_tiles<KEYS>(p, q);
-      const int before = packed_count(t, lo + 1), here = packed_count(t, lo) - before;
+      const int before = packed_count(t, lo + 1), here = (packed_count(t, lo) - before) * P;
       const int upto = wave_scan_i32(here), sum = __builtin_amdgcn_readlane(upto, 63);
       if (left < sum) {
         const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > left));
-        const int u = __builtin_amdgcn_readlane(before, who) + left -
-                      (__builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(here, who));
+        const int in = left - (__builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(here, who));
+        const int u = __builtin_amdgcn_readlane(before, who) + in / P;
         r.s = PackedSeq{__builtin_amdgcn_readlane(q.qb, who), __builtin_amdgcn_readlane(q.nq, who),
                         __builtin_amdgcn_readlane(q.kb, who), __builtin_amdgcn_readlane(q.nk, who)};
         r.tile = KEYS || !p.causal ? u : __builtin_amdgcn_readlane(t.tiles, who) - 1 - u;
+        r.parts = P;
+        r.part = in % P;
         break;
       }
       left -= sum;
@@ -152,14 +204,14 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
 }
 
 // Zeros for the rows outside every sequence, 128-row pieces dealt to the spare workgroups (there is one at least
-// whenever there is such a row: the grid has ceil(rows / 128) + n tiles).
+// whenever there is such a row: packed_grid).
 template <class T, int D>
 __device__ __forceinline__ void packed_zero_rest(T* rows, int64_t sn, const int32_t* off, int n, int total, int which,
                                                  int spare) {
   static_assert(sizeof(T) == 2, "16-bit rows");
   constexpr int CH = D / 8;
   const int first = min(max(off[0], 0), total), last = min(max(off[n], 0), total);
-  for (int r0 = which * kPackedTile; r0 < total; r0 += spare * kPackedTile)
+  for (int r0 = max(which, 0) * kPackedTile; r0 < total; r0 += max(spare, 1) * kPackedTile)
     for (int i = threadIdx.x; i < kPackedTile * CH; i += (int)blockDim.x) {
       const int r = r0 + i / CH;
       if (r < total && (r < first || r >= last)) *(uint4*)((char*)(rows + r * sn) + (i % CH) * 16) = uint4{0, 0, 0, 0};
@@ -251,8 +303,20 @@ __device__ __forceinline__ int packed_head(int pos, int heads) {
   return (pos % g) * (heads / g) + pos / g;
 }
 
+// Workgroups of a launch with `heads` of a tile each: every tile (a partial one a sequence), the parts of split ones, and one
+// spare at least wherever a row is of no sequence.
+inline int64_t packed_grid(int rows, int n, int heads, bool split) {
+  const int64_t tiles = (int64_t)(rows + kPackedTile - 1) / kPackedTile + n;
+  return (tiles + (split ? (kPackedParts + heads - 1) / heads : 0)) * heads;
+}
+// Whether tiles are split: long sequences on average, some of them with more than kPackedSplit units.  (Offsets are on the
+// GPU: the host sees the sums alone.  In a batch of short prompts, 12 of 40 to 2900 tokens, parts and their sums cost more
+// than the balance gives: 65.8 -> 82 us.)
+constexpr int kPackedSplit = 24;
+inline bool packed_splits(int64_t others, int n) { return others > kPackedSplit * kPackedTile && others >= 2048ll * n; }
+
 int packed_fwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);
 int packed_bwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);
-int packed_bwd_splits(int64_t tk, int n, int kv_heads, int group);
+int packed_bwd_splits(int64_t tk, int kv_heads, int group);
 
 }  // namespace vmo

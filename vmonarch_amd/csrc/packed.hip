@@ -27,7 +27,7 @@ static int packed_prepare(const vmo_packed_args* a, bool bwd, const char* what, 
     }
   if (bwd && a->tq > 0 && !a->lse) return set_error(VMO_ERR_INVALID, "%s: needs the forward's lse", what);
   const int64_t tiles = ((int64_t)(a->tq > a->tk ? a->tq : a->tk) + kPackedTile - 1) / kPackedTile + a->n;
-  if (a->tq > (1 << 30) || a->tk > (1 << 30) || tiles * a->heads > (1ll << 30))
+  if (a->tq > (1 << 26) || a->tk > (1 << 26) || tiles * a->heads > (1ll << 30))   // (counts of tiles stay within 32 bits)
     return set_error(VMO_ERR_UNSUPPORTED, "%s: too many rows", what);
   PackedParams p{};
   p.q = a->q.data; p.k = a->k.data; p.v = a->v.data; p.o = p.out = a->o.data; p.dO = a->grad_o.data;
@@ -47,44 +47,69 @@ static int packed_prepare(const vmo_packed_args* a, bool bwd, const char* what, 
   return VMO_OK;
 }
 
-// Workspace of the backward: -delta, then the parts of dk and of dv.
-static int64_t bwd_layout(const vmo_packed_args* a, int* splits, int64_t* delta_floats) {
-  *splits = packed_bwd_splits(a->tk, a->n, a->kv_heads, a->heads / a->kv_heads);
-  *delta_floats = ((int64_t)a->heads * a->tq + 63) / 64 * 64;
-  return (*delta_floats + (*splits > 1 ? 2ll * *splits * a->kv_heads * a->tk * a->d : 0)) * 4;
+// Workspaces: the parts of split tiles (the forward's with their m and l, the backward's of dq, then of dk and dv), and
+// before them the backward's -delta.  Some slots more than kPackedParts: parts come in whole heads.
+static int64_t part_floats(int d, int heads) { return (int64_t)(kPackedParts + heads) * kPackedTile * d; }
+static int64_t fwd_layout(const vmo_packed_args* a) {
+  return packed_splits(a->tk, a->n) ? (part_floats(a->d, a->heads) + part_floats(2, a->heads)) * 4 : 0;
+}
+struct BwdLayout { int64_t delta, kv, bytes; int splits; };   // floats of -delta and of dk's parts
+static BwdLayout bwd_layout(const vmo_packed_args* a) {
+  BwdLayout l;
+  l.delta = ((int64_t)a->heads * a->tq + 63) / 64 * 64;
+  l.splits = packed_bwd_splits(a->tk, a->kv_heads, a->heads / a->kv_heads);
+  const int64_t q = packed_splits(a->tk, a->n) ? part_floats(a->d, a->heads) : 0;
+  l.kv = l.splits > 1 ? (int64_t)l.splits * a->kv_heads * a->tk * a->d
+         : packed_splits(a->tq, a->n) ? part_floats(a->d, a->kv_heads) : 0;
+  l.bytes = (l.delta + (q > 2 * l.kv ? q : 2 * l.kv)) * 4;
+  return l;
+}
+static bool sizes_ok(const vmo_packed_args* a) {
+  return a && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->n >= 0 && a->tq >= 0 && a->tk >= 0 && (a->d == 64 || a->d == 128);
+}
+static int workspace_check(const vmo_packed_args* a, int64_t need, const char* what) {
+  if (need > 0 && (!a->workspace || a->workspace_bytes < (size_t)need || !aligned16(a->workspace)))
+    return set_error(VMO_ERR_WORKSPACE, "%s: needs %lld workspace bytes, has %llu", what, (long long)need,
+                     (unsigned long long)(a->workspace ? a->workspace_bytes : 0));
+  return VMO_OK;
 }
 
 }  // namespace vmo
+
+extern "C" size_t vmo_packed_fwd_workspace_size(const vmo_packed_args* a) { return vmo::sizes_ok(a) ? (size_t)vmo::fwd_layout(a) : 0; }
 
 extern "C" int vmo_packed_fwd(const vmo_packed_args* a, void* stream) {
   using namespace vmo;
   clear_error();
   PackedParams p;
-  const int rc = packed_prepare(a, false, "packed_fwd", &p);
+  int rc = packed_prepare(a, false, "packed_fwd", &p);
   if (rc != VMO_OK || a->tq == 0) return rc;
+  rc = workspace_check(a, fwd_layout(a), "packed_fwd");
+  if (rc != VMO_OK) return rc;
+  if (packed_splits(a->tk, a->n)) {
+    p.split_least = kPackedSplit;
+    p.part = (float*)a->workspace;
+    p.part2 = p.part + part_floats(a->d, a->heads);
+  }
   return packed_fwd_launch(p, a->dtype == VMO_DTYPE_F16, a->d, (hipStream_t)stream);
 }
 
 extern "C" size_t vmo_packed_bwd_workspace_size(const vmo_packed_args* a) {
-  if (!a || a->heads <= 0 || a->kv_heads <= 0 || a->tq < 0 || a->tk < 0) return 0;
-  int splits;
-  int64_t delta;
-  return (size_t)vmo::bwd_layout(a, &splits, &delta);
+  return vmo::sizes_ok(a) ? (size_t)vmo::bwd_layout(a).bytes : 0;
 }
 
 extern "C" int vmo_packed_bwd(const vmo_packed_args* a, void* stream) {
   using namespace vmo;
   clear_error();
   PackedParams p;
-  const int rc = packed_prepare(a, true, "packed_bwd", &p);
+  int rc = packed_prepare(a, true, "packed_bwd", &p);
   if (rc != VMO_OK || (a->tq == 0 && a->tk == 0)) return rc;
-  int64_t delta;
-  const int64_t need = bwd_layout(a, &p.splits, &delta);
-  if (need > 0 && (!a->workspace || a->workspace_bytes < (size_t)need || !aligned16(a->workspace)))
-    return set_error(VMO_ERR_WORKSPACE, "packed_bwd: needs %lld workspace bytes, has %llu", (long long)need,
-                     (unsigned long long)(a->workspace ? a->workspace_bytes : 0));
+  const BwdLayout l = bwd_layout(a);
+  rc = workspace_check(a, l.bytes, "packed_bwd");
+  if (rc != VMO_OK) return rc;
+  p.splits = l.splits;
   p.neg_delta = (float*)a->workspace;
-  p.dk_part = p.neg_delta + delta;
-  p.dv_part = p.dk_part + (int64_t)p.splits * a->kv_heads * a->tk * a->d;
+  p.part = p.neg_delta + l.delta;
+  p.part2 = p.part + l.kv;
   return packed_bwd_launch(p, a->dtype == VMO_DTYPE_F16, a->d, (hipStream_t)stream);
 }

@@ -7,7 +7,8 @@
 //    the diagonal, then dQ^T += K^T dS^T.  Its prologue forms delta.
 //  * packed_bwd_dkdv: 128 keys of one key / value head, 32 a wave, one a lane; over 32-query stages from the diagonal on,
 //    for one query head of the group after the other, S = Q K^T and dP = dO V^T, then dV^T += dO^T P, dK^T += Q^T dS.
-//    With few key tiles the group's heads are split over several workgroups, whose fp32 parts packed_bwd_sum adds in order.
+// Where some workgroups have far more to do than others, heavy tiles are split (packed.h; dk / dv: over the group's heads
+// first), into fp32 sums that packed_bwd_join (or packed_bwd_sum) adds in order.
 // Stages that a wave does not see at all are skipped, those on the diagonal (or at a sequence's end) masked.
 // P and dS are rounded to the 16-bit type as operands, the gradients once at the end.
 #include "packed.h"
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
   auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
 
   const int head = uni(packed_head((int)blockIdx.x % p.heads, p.heads));
-  const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, (VMO_LDS int*)smem);
+  const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, p.heads, (VMO_LDS int*)smem);
   if (w.tile < 0) {
     packed_zero_rest<T, D>((T*)p.dq + head * p.dq_sh, p.dq_sn, p.q_off, p.n, p.tq, w.which, w.spare);
     return;
@@ -64,7 +65,8 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
   const int row = min(q0 + l32, nq - 1);
   const int lim = keys_of(row);
   const int lo = uni(keys_of(min(q0, nq - 1))), hi = uni(keys_of(min(q0 + 31, nq - 1)));
-  const int n_tiles = uni((keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 1, nq - 1)) + kDqKeys - 1) / kDqKeys);
+  const int stages = uni((keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 1, nq - 1)) + kDqKeys - 1) / kDqKeys);
+  const int parts = uni(w.parts), t0 = uni((int)((int64_t)w.part * stages / parts)), t1 = uni((int)((int64_t)(w.part + 1) * stages / parts));
 
   // Q^T and dO^T as B operands (one query a lane); delta in fp32
   V8 qf[NDS], dof[NDS];
@@ -91,7 +93,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
   float alpha = -wave_sum32(delta);
   float lse = p.lse[(int64_t)head * p.st_sh + tok];
   asm volatile("" : "+v"(alpha), "+v"(lse));   // waited for here: a wait in the loop would also wait for the copies
-  if (live && hl == 0 && q0 + l32 < nq) p.neg_delta[(int64_t)head * p.tq + tok] = alpha;
+  if (live && w.part == 0 && hl == 0 && q0 + l32 < nq) p.neg_delta[(int64_t)head * p.tq + tok] = alpha;
 
   const T* kbase = (const T*)p.k + (int64_t)(head / p.group) * p.k_sh + (int64_t)kb * p.k_sn;
   const T* vbase = (const T*)p.v + (int64_t)(head / p.group) * p.v_sh + (int64_t)kb * p.v_sn;
@@ -157,28 +159,33 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
           });
     }
   };
-  if (n_tiles > 0) {
-    issue(0);
-    const int n_full = live ? uni(min(lo / kDqKeys, n_tiles)) : 0;
+  if (t1 > t0) {
+    issue(t0);
+    const int n_full = live ? uni(min(max(lo / kDqKeys, t0), t1)) : t0;
     auto top = [&](int t) __attribute__((always_inline)) {
       tile_sync<0>();   // stage t has landed for every wave, and stage t - 1's slot is free
-      if (t + 1 < n_tiles) issue(t + 1);
+      if (t + 1 < t1) issue(t + 1);
     };
-    int t = 0;
+    int t = t0;
     for (; t < n_full; ++t) {
       top(t);
       stage(t, std::false_type{});
     }
-    for (; t < n_tiles; ++t) {
+    for (; t < t1; ++t) {
       top(t);
       if (live && t * kDqKeys < hi) stage(t, std::true_type{});
     }
   }
   __syncthreads();
   if (!live) return;
+  VMO_LDS float* patch = (VMO_LDS float*)(smem + wave * kEpiPatchBytes);
+  if (parts > 1) {
+    float* out = p.part + ((int64_t)blockIdx.x * kPackedTile + wave * 32) * D;
+    store_acc_rows<F16>(patch, acc, NA, p.sm_scale, kGradStoreF32, (char*)out, D * 4, min(32, nq - q0), lane);
+    return;
+  }
   T* out = (T*)p.dq + (int64_t)head * p.dq_sh + (int64_t)(qb + q0) * p.dq_sn;
-  store_acc_rows<F16>((VMO_LDS float*)(smem + wave * kEpiPatchBytes), acc, NA, p.sm_scale, kGradStore, (char*)out, p.dq_sn * 2,
-                      min(32, nq - q0), lane);
+  store_acc_rows<F16>(patch, acc, NA, p.sm_scale, kGradStore, (char*)out, p.dq_sn * 2, min(32, nq - q0), lane);
 }
 
 template <bool F16, int D>
@@ -194,10 +201,10 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   const uint32_t smem_u32 = (uint32_t)(uintptr_t)smem;
   auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
 
-  const int shares = p.kv_heads * p.splits;   // workgroups of one key tile
+  const int shares = p.kv_heads * p.splits;   // workgroups of one key tile (a share stays on its XCDs, so its heads' rows do)
   const int hs = uni(packed_head((int)blockIdx.x % shares, shares));
   const int kvh = hs / p.splits, split = hs % p.splits;
-  const PackedTile w = packed_locate<true>(p, (int)blockIdx.x / shares, (int)gridDim.x / shares, (VMO_LDS int*)smem);
+  const PackedTile w = packed_locate<true>(p, (int)blockIdx.x / shares, (int)gridDim.x / shares, shares, (VMO_LDS int*)smem);
   if (w.tile < 0) {
     if (p.splits == 1) {
       packed_zero_rest<T, D>((T*)p.dk + kvh * p.dk_sh, p.dk_sn, p.k_off, p.n, p.tk, w.which, w.spare);
@@ -216,8 +223,13 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   const int from = first_row(key);
   const int w_from = uni(first_row(min(k0, nk - 1))), w_whole = uni(first_row(min(k0 + 31, nk - 1)));
   const int t0 = uni(first_row(tile0) / kKvQueries), t1 = uni((nq + kKvQueries - 1) / kKvQueries);
-  const int per = p.group / p.splits, h0 = kvh * p.group + split * per;
-  const int steps = t1 > t0 ? t1 - t0 : 0, n_it = uni(steps * per);
+  // the share's heads; the part's steps of all (head, stage) pairs: from stage b0 of head g0 up to stage b1 of head g1
+  const int per = p.group / p.splits;
+  const int steps = t1 > t0 ? t1 - t0 : 0, parts = uni(w.parts);
+  const int64_t all = (int64_t)steps * per;
+  const int i0 = uni((int)(w.part * all / parts)), i1 = uni((int)((w.part + 1) * all / parts)), n_it = i1 - i0;
+  const int g0 = steps ? uni(i0 / steps) : 0, g1 = steps ? uni((i1 - 1) / steps) : -1, h0 = kvh * p.group + split * per + g0;
+  const int b0 = t0 + i0 - g0 * steps, b1 = t0 + i1 - g1 * steps;
 
   const T* kp0 = (const T*)p.k + (int64_t)kvh * p.k_sh + (int64_t)kb * p.k_sn;
   const T* vp0 = (const T*)p.v + (int64_t)kvh * p.v_sh + (int64_t)kb * p.v_sn;
@@ -244,7 +256,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
                                                      lane);
   const float* lse_h = p.lse + (int64_t)h0 * p.st_sh + qb;
   const float* nd_h = p.neg_delta + (int64_t)h0 * p.tq + qb;
-  int t_next = t0;   // the stage that the next issue copies; past the last one comes the next head's first
+  int t_next = b0;   // the stage that the next issue copies; past the last one comes the next head's first
   auto issue = [&](int slot) __attribute__((always_inline)) {
     const uint32_t st = smem_u32 + (uint32_t)(slot * STAGE);
     const int row0 = t_next * kKvQueries;
@@ -352,16 +364,16 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
       if (live && (t + 1) * kKvQueries > w_from) stage(it & 1, t * kKvQueries, std::true_type{});
       ++it;
     };
-    for (int h = 0; h < per; ++h) {
-      int t = t0;
-      const int upto = live ? a0 : t1;
-      for (; t < upto; ++t) masked(t);
-      for (; t < a1; ++t) {
+    for (int g = g0; g <= g1; ++g) {
+      int t = g == g0 ? b0 : t0;
+      const int end = g == g1 ? b1 : t1;
+      for (const int upto = live ? min(a0, end) : end; t < upto; ++t) masked(t);
+      for (const int upto = min(a1, end); t < upto; ++t) {
         top();
         stage(it & 1, t * kKvQueries, std::false_type{});
         ++it;
       }
-      for (; t < t1; ++t) masked(t);
+      for (; t < end; ++t) masked(t);
     }
   } else {
     tile_sync<0>();   // V's copies have landed before the patches take their place
@@ -370,10 +382,10 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   if (!live) return;
   VMO_LDS float* patch = (VMO_LDS float*)(smem + wave * kEpiPatchBytes);
   const int nrows = min(32, nk - k0);
-  if (p.splits > 1) {
-    const int64_t r = ((int64_t)(split * p.kv_heads + kvh) * p.tk + kb + k0) * D;
-    store_acc_rows<F16>(patch, dk, NA, p.sm_scale, kGradStoreF32, (char*)(p.dk_part + r), D * 4, nrows, lane);
-    store_acc_rows<F16>(patch, dv, NA, 1.0f, kGradStoreF32, (char*)(p.dv_part + r), D * 4, nrows, lane);
+  if (parts > 1 || p.splits > 1) {
+    const int64_t r = (p.splits > 1 ? (int64_t)(split * p.kv_heads + kvh) * p.tk + kb + k0 : (int64_t)blockIdx.x * kPackedTile + wave * 32) * D;
+    store_acc_rows<F16>(patch, dk, NA, p.sm_scale, kGradStoreF32, (char*)(p.part + r), D * 4, nrows, lane);
+    store_acc_rows<F16>(patch, dv, NA, 1.0f, kGradStoreF32, (char*)(p.part2 + r), D * 4, nrows, lane);
   } else {
     store_acc_rows<F16>(patch, dk, NA, p.sm_scale, kGradStore,
                         (char*)((T*)p.dk + (int64_t)kvh * p.dk_sh + (int64_t)(kb + k0) * p.dk_sn), p.dk_sn * 2, nrows, lane);
@@ -382,7 +394,45 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   }
 }
 
-// dk and dv from their parts, in the parts' order; rows outside every sequence (they have no parts) are zeros.
+// dq, or dk and dv, of split tiles from their parts, in the parts' order: the workgroup of part k takes its share of the
+// tile's rows, D / 4 lanes a row.
+template <bool F16, int D, bool KEYS>
+__global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams p) {
+  using T = typename Elem<F16>::T;
+  using V4 = typename Elem<F16>::V4;
+  constexpr int TPR = D / 4;
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  const int heads = KEYS ? p.kv_heads : p.heads, head = packed_head((int)blockIdx.x % heads, heads);
+  const PackedTile w = packed_locate<KEYS>(p, (int)blockIdx.x / heads, 1 << 20, heads, (VMO_LDS int*)(VMO_LDS char*)smem_raw);
+  if (w.tile < 0 || w.parts == 1) return;
+  const int rows = min(kPackedTile, (KEYS ? w.s.nk : w.s.nq) - w.tile * kPackedTile), d4 = (threadIdx.x % TPR) * 4;
+  const int64_t slot0 = (int)blockIdx.x - w.part * heads;
+  for (int r = w.part * rows / w.parts + threadIdx.x / TPR; r < (w.part + 1) * rows / w.parts; r += 256 / TPR) {
+    f32x4 a = f32x4{}, b = f32x4{};
+#pragma unroll 4
+    for (int i = 0; i < w.parts; ++i) {
+      const int64_t at = ((slot0 + i * heads) * kPackedTile + r) * D + d4;
+      a += *(const f32x4*)(p.part + at);
+      if constexpr (KEYS) b += *(const f32x4*)(p.part2 + at);
+    }
+    V4 x, y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = to_elem<T>(a[e]);
+      y[e] = to_elem<T>(b[e]);
+    }
+    const int64_t tok = (KEYS ? w.s.kb : w.s.qb) + w.tile * kPackedTile + r;
+    if constexpr (KEYS) {
+      *(V4*)((T*)p.dk + (int64_t)head * p.dk_sh + tok * p.dk_sn + d4) = x;
+      *(V4*)((T*)p.dv + (int64_t)head * p.dv_sh + tok * p.dv_sn + d4) = y;
+    } else {
+      *(V4*)((T*)p.dq + (int64_t)head * p.dq_sh + tok * p.dq_sn + d4) = x;
+    }
+  }
+}
+
+// dk and dv from the sums of workgroups that had some of the group's heads each, in their order; rows outside every sequence
+// (they have no sums) are zeros.
 template <bool F16, int D>
 __global__ __launch_bounds__(256) void packed_bwd_sum_kernel(PackedParams p) {
   using T = typename Elem<F16>::T;
@@ -395,10 +445,11 @@ __global__ __launch_bounds__(256) void packed_bwd_sum_kernel(PackedParams p) {
   const int kvh = (int)(r / p.tk), tok = (int)(r % p.tk);
   f32x4 a = f32x4{}, b = f32x4{};
   if (tok >= min(max(p.k_off[0], 0), p.tk) && tok < min(max(p.k_off[p.n], 0), p.tk))
+#pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
       const int64_t at = (s * rows + r) * D + c4;
-      a += *(const f32x4*)(p.dk_part + at);
-      b += *(const f32x4*)(p.dv_part + at);
+      a += *(const f32x4*)(p.part + at);
+      b += *(const f32x4*)(p.part2 + at);
     }
   V4 x, y;
 #pragma unroll
@@ -410,12 +461,13 @@ __global__ __launch_bounds__(256) void packed_bwd_sum_kernel(PackedParams p) {
   *(V4*)((T*)p.dv + (int64_t)kvh * p.dv_sh + (int64_t)tok * p.dv_sn + c4) = y;
 }
 
-// Workgroups that share a key tile: as many as divide the group and bring the launch to two rounds of the chip's slots
-// (256 CUs, two workgroups each).
-int packed_bwd_splits(int64_t tk, int n, int kv_heads, int group) {
+// Workgroups that share a key tile: as many as divide the group and bring the launch to two rounds of the chip's slots.  With
+// shared heads this balances better than parts of a tile do, whose queries every XCD's L2 would have to hold (8 heads over 2,
+// prompts of 12000 and 4384 tokens: 651 us so, 790 in parts).
+int packed_bwd_splits(int64_t tk, int kv_heads, int group) {
   const int64_t tiles = ((tk + kPackedTile - 1) / kPackedTile) * kv_heads;
   int splits = 1;
-  while (splits < group && tiles * splits < 1024) {
+  while (splits < group && tiles * splits < 2 * kPackedSlots) {
     int next = splits + 1;
     while (group % next) ++next;
     splits = next;
@@ -424,13 +476,21 @@ int packed_bwd_splits(int64_t tk, int n, int kv_heads, int group) {
 }
 
 template <bool F16, int D>
-static int launch_packed_bwd(const PackedParams& p, hipStream_t s) {
+static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   constexpr int LDS_Q = packed_dq_lds<D>(), LDS_KV = packed_kv_lds<D>();
   static_assert(LDS_Q <= 65536 && LDS_KV <= 80 * 1024, "two workgroups a CU");
+  auto join = [&](auto kern, int heads) {
+    const int64_t slots = (kPackedParts + heads - 1) / heads * heads;
+    hipLaunchKernelGGL(kern, dim3((unsigned)slots), dim3(256), kPackedSeqBytes * kPackedMaxSeqs, s, p);
+    return launch_status("packed_bwd_join");
+  };
+  int rc = VMO_OK;
   if (p.tq > 0) {
-    const int64_t grid = ((int64_t)(p.tq + kPackedTile - 1) / kPackedTile + p.n) * p.heads;
+    p.split_least = packed_splits(p.tk, p.n) ? kPackedSplit : 0;
+    const int64_t grid = packed_grid(p.tq, p.n, p.heads, p.split_least > 0);
     hipLaunchKernelGGL((packed_bwd_dq_kernel<F16, D>), dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_Q, s, p);
-    const int rc = launch_status("packed_bwd_dq");
+    rc = launch_status("packed_bwd_dq");
+    if (rc == VMO_OK && p.split_least > 0) rc = join(packed_bwd_join_kernel<F16, D, false>, p.heads);
     if (rc != VMO_OK) return rc;
   }
   if (p.tk == 0) return VMO_OK;
@@ -438,10 +498,13 @@ static int launch_packed_bwd(const PackedParams& p, hipStream_t s) {
   if (LDS_KV > 65536 &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_KV) != hipSuccess)
     return set_error(VMO_ERR_LAUNCH, "packed_bwd: cannot raise the LDS limit to %d bytes", LDS_KV);
-  const int64_t grid = ((int64_t)(p.tk + kPackedTile - 1) / kPackedTile + p.n) * p.kv_heads * p.splits;
+  p.split_least = p.splits == 1 && packed_splits(p.tq, p.n) ? kPackedSplit : 0;
+  const int64_t grid = packed_grid(p.tk, p.n, p.kv_heads * p.splits, p.split_least > 0);
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_KV, s, p);
-  const int rc = launch_status("packed_bwd_dkdv");
-  if (rc != VMO_OK || p.splits == 1) return rc;
+  rc = launch_status("packed_bwd_dkdv");
+  if (rc != VMO_OK) return rc;
+  if (p.split_least > 0) return join(packed_bwd_join_kernel<F16, D, true>, p.kv_heads);
+  if (p.splits == 1) return VMO_OK;
   const int64_t threads = (int64_t)p.kv_heads * p.tk * (D / 4);
   hipLaunchKernelGGL((packed_bwd_sum_kernel<F16, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
   return launch_status("packed_bwd_sum");

@@ -17,6 +17,7 @@
 //  * where the launch is small, eight waves share the 128 queries: two groups of four take every other stage, each with a
 //    ring of its own, and the second's sums join the first's in LDS (G = 2).
 // The row sums add the fp32 p; p is rounded to the 16-bit type as the operand of P V, o once at the end.
+#include <stdlib.h>
 #include "packed.h"
 
 namespace vmo {
@@ -46,7 +47,7 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
   auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
 
   const int head = uni(packed_head((int)blockIdx.x % p.heads, p.heads));
-  const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, (VMO_LDS int*)smem);
+  const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, p.heads, (VMO_LDS int*)smem);
   if (w.tile < 0) {
     if (p.zero_rest)
       packed_zero_rest<T, D>((T*)p.out + head * p.o_sh, p.o_sn, p.q_off, p.n, p.tq, w.which, w.spare);
@@ -65,9 +66,11 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
   const int row = min(q0 + l32, nq - 1);
   const int lim = keys_of(row);
   const int lo = uni(keys_of(min(q0, nq - 1))), hi = uni(keys_of(min(q0 + 31, nq - 1)));   // least and most of the wave
-  const int all_tiles = uni((keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 1, nq - 1)) + kFwdBN - 1) / kFwdBN);
-
-  const int n_tiles = G > 1 ? (all_tiles - grp + G - 1) / G : all_tiles, steps = (all_tiles + G - 1) / G;   // the group's tiles
+  // the part's stages, from `begin` on, and those of them that the key group takes
+  const int stages = uni((keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 1, nq - 1)) + kFwdBN - 1) / kFwdBN);
+  const int parts = uni(w.parts), begin = uni((int)((int64_t)w.part * stages / parts)) + grp;
+  const int all_tiles = uni((int)((int64_t)(w.part + 1) * stages / parts)) + grp - begin;
+  const int n_tiles = G > 1 ? (all_tiles - grp + G - 1) / G : all_tiles, steps = (all_tiles + G - 1) / G;
 
   const T* kbase = (const T*)p.k + (int64_t)(head / p.group) * p.k_sh + (int64_t)kb * p.k_sn;
   const T* vbase = (const T*)p.v + (int64_t)(head / p.group) * p.v_sh + (int64_t)kb * p.v_sn;
@@ -76,8 +79,8 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
     uint32_t sb = ring_u32;
     asm volatile("" : "+s"(sb));
     const uint32_t st = sb + (uint32_t)((t % NSLOT) * STAGE);
-    kcopy.issue((t * G + grp) * kFwdBN, nk, st);   // (a tile that runs past the sequence repeats its last key: masked)
-    vcopy.issue((t * G + grp) * kFwdBN, nk, st + K_BYTES);
+    kcopy.issue((begin + t * G) * kFwdBN, nk, st);   // (a tile that runs past the sequence repeats its last key: masked)
+    vcopy.issue((begin + t * G) * kFwdBN, nk, st + K_BYTES);
   };
 
   auto prime = [&]() __attribute__((always_inline)) {
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
   // Tile t sits in ring slot t % NSLOT; at its top this wave's copies of it have landed (only those of tile t + 1 may be
   // under way), after the barrier every wave's have, and the slot of tile t - 1 is free for tile t + NSLOT - 1.
   constexpr int kSteadyPending = NSLOT == 3 ? DMA_PER_TILE : 0;
-  const int n_full = live ? uni(min((lo / kFwdBN - grp + G - 1) / G, n_tiles)) : 0;
+  const int n_full = live ? uni(min(max((lo / kFwdBN - begin + G - 1) / G, 0), n_tiles)) : 0;
   auto top = [&](int t) __attribute__((always_inline)) {
     if (NSLOT == 3 && t + 1 < n_tiles) tile_sync<kSteadyPending>();
     else tile_sync<0>();
@@ -262,7 +265,7 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
     }
     for (; t < steps; ++t) {
       top(t);
-      const int key0 = (t * G + grp) * kFwdBN;
+      const int key0 = (begin + t * G) * kFwdBN;
       if (live && key0 < hi) masked_stage(slot(t), key0);
     }
     __syncthreads();   // the ring is free
@@ -307,13 +310,57 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
     // (each wave's row patch lies in its own box)
   }
   if (!live) return;
-  const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;   // (a row that sees no key)
   const int nrows = min(32, nq - q0);
+  VMO_LDS float* patch = (VMO_LDS float*)(smem + wave * (G > 1 ? (NA * 16 + 2) * 256 : kEpiPatchBytes));
+  if (parts > 1) {
+    const int64_t at = (int64_t)blockIdx.x * kPackedTile + wave * 32;
+    store_acc_rows<F16>(patch, acc, NA, 1.f, kGradStoreF32, (char*)(p.part + at * D), D * 4, nrows, lane);
+    if (hl == 0 && l32 < nrows) {
+      p.part2[2 * (at + l32)] = m_run;
+      p.part2[2 * (at + l32) + 1] = l_tot;
+    }
+    return;
+  }
+  const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;   // (a row that sees no key)
   T* out = (T*)p.out + (int64_t)head * p.o_sh + (int64_t)(qb + q0) * p.o_sn;
-  store_acc_rows<F16>((VMO_LDS float*)(smem + wave * (G > 1 ? (NA * 16 + 2) * 256 : kEpiPatchBytes)), acc, NA, inv, kGradStore, (char*)out, p.o_sn * 2, nrows,
-                      lane);
+  store_acc_rows<F16>(patch, acc, NA, inv, kGradStore, (char*)out, p.o_sn * 2, nrows, lane);
   if (p.lse && hl == 0 && l32 < nrows)
     p.lse[(int64_t)head * p.st_sh + qb + q0 + l32] = l_tot == 0.f ? 0.f : m_run + fast_log2(l_tot);
+}
+
+// o (and lse) of split tiles from their parts: the workgroup of part k takes its share of the tile's rows, D / 4 lanes a row.
+template <bool F16, int D>
+__global__ __launch_bounds__(256) void packed_fwd_join_kernel(PackedParams p) {
+  using T = typename Elem<F16>::T;
+  constexpr int TPR = D / 4;
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  const int head = packed_head((int)blockIdx.x % p.heads, p.heads);
+  const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, 1 << 20, p.heads, (VMO_LDS int*)(VMO_LDS char*)smem_raw);
+  if (w.tile < 0 || w.parts == 1) return;
+  const int rows = min(kPackedTile, w.s.nq - w.tile * kPackedTile), d4 = (threadIdx.x % TPR) * 4;
+  const int slot0 = (int)blockIdx.x - w.part * p.heads;
+  for (int r = w.part * rows / w.parts + threadIdx.x / TPR; r < (w.part + 1) * rows / w.parts; r += 256 / TPR) {
+    float m = kNoMax, l = 0.f;
+    f32x4 acc = f32x4{};
+#pragma unroll 4
+    for (int i = 0; i < w.parts; ++i) {
+      const int64_t at = (int64_t)(slot0 + i * p.heads) * kPackedTile + r;
+      const float pm = p.part2[2 * at], pl = p.part2[2 * at + 1];
+      const f32x4 y = *(const f32x4*)(p.part + at * D + d4);
+      const float m_new = fmaxf(m, pm), f = fast_exp2(m - m_new), pf = fast_exp2(pm - m_new);
+      m = m_new;
+      l = fmaf(l, f, pl * pf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(acc[e], f, y[e] * pf);
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    typename Elem<F16>::V4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = to_elem<T>(acc[e] * inv);
+    const int64_t tok = w.s.qb + w.tile * kPackedTile + r;
+    *(typename Elem<F16>::V4*)((T*)p.out + (int64_t)head * p.o_sh + tok * p.o_sn + d4) = y;
+    if (p.lse && d4 == 0) p.lse[(int64_t)head * p.st_sh + tok] = l == 0.f ? 0.f : m + fast_log2(l);
+  }
 }
 
 template <bool F16, int D, int G>
@@ -327,14 +374,18 @@ static int launch_packed_fwd(const PackedParams& p, int64_t grid, hipStream_t s)
 }
 
 template <bool F16, int D>
-static int dispatch_packed_fwd(const PackedParams& p, hipStream_t s) {
-  const int64_t grid = ((int64_t)(p.tq + kPackedTile - 1) / kPackedTile + p.n) * p.heads;
+static int dispatch_packed_fwd(PackedParams p, hipStream_t s) {
+  const int64_t grid = packed_grid(p.tq, p.n, p.heads, p.split_least > 0);
   // Two key groups halve the longest workgroup's time, which is the launch's where the chip holds all of them at once (one
-  // prompt of 4096 tokens, 12 heads of 128: 80.2 -> 65.7 us, of 2048: 38.8 -> 34.7); with more workgroups, the barriers
-  // that eight waves share cost (8192 tokens 214.6 -> 224.4 us), and for short prompts the join does (four of up to 200
-  // tokens, 64 wide: 8.9 -> 9.6 us).
-  const bool two = grid <= 512 && p.tk >= 768ll * p.n;
-  return two ? launch_packed_fwd<F16, D, 2>(p, grid, s) : launch_packed_fwd<F16, D, 1>(p, grid, s);
+  // prompt of 2048 tokens, 12 heads of 128: 38.8 -> 34.7 us; of 4096, 80.2 -> 65.7, where splitting tiles gives @@); with
+  // more workgroups, the barriers that eight waves share cost (8192 tokens 214.6 -> 224.4 us), and for short prompts the
+  // join does (four of up to 200 tokens, 64 wide: 8.9 -> 9.6 us).
+  const bool two = getenv("PG") ? atoi(getenv("PG")) == 2 : p.split_least == 0 && grid <= 512 && p.tk >= 768ll * p.n;
+  const int rc = two ? launch_packed_fwd<F16, D, 2>(p, grid, s) : launch_packed_fwd<F16, D, 1>(p, grid, s);
+  if (rc != VMO_OK || p.split_least == 0) return rc;
+  const int64_t slots = (kPackedParts + p.heads - 1) / p.heads * p.heads;
+  hipLaunchKernelGGL((packed_fwd_join_kernel<F16, D>), dim3((unsigned)slots), dim3(256), kPackedSeqBytes * kPackedMaxSeqs, s, p);
+  return launch_status("packed_fwd_join");
 }
 
 int packed_fwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s) {
