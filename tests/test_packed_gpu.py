@@ -37,6 +37,11 @@ CASES = [
     ([40, 129, 9], [200, 65, 0], 2, 2, 128, "bf16", "hnd", False),
     ([0, 0], None, 2, 1, 64, "bf16", "hnd", True),
     ([5] * 70 + [150], None, 2, 1, 64, "f16", "nhd", True),             # more sequences than lanes
+    ([3000], None, 2, 1, 64, "f16", "nhd", True),                       # two key groups
+    ([2000, 1300], None, 2, 2, 128, "bf16", "hnd", False),
+    ([7000], None, 1, 1, 64, "bf16", "hnd", True),                      # heavy tiles in parts
+    ([6500, 77], [7100, 77], 2, 2, 128, "bf16", "nhd", True),
+    ([6200], None, 2, 1, 128, "f16", "hnd", False),
 ]
 
 

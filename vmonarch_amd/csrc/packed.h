@@ -82,30 +82,26 @@ __device__ __forceinline__ int packed_count(const PackedTiles& t, int level) {
   return level <= t.cap ? min(max(t.top - level + 1, 0), t.tiles) : 0;
 }
 
-// Heavy tiles are split: one long prompt's last tile sees all its keys, and alone took longer than the average workgroup slot
-// has work (8 heads of 128, prompts of 12000 and 4384 tokens: 188 stages of a mean of 78, and the CUs idle 29 % of the
-// forward; split, it takes 336 us instead of 372, dq 470 instead of 500).  A tile of more than S units is cut into
-// ceil(L / S) parts of equal length, S the mean work of the chip's kPackedSlots workgroups (smaller parts balance no better:
-// their sums' traffic grows; 336 -> 357 us with half of S) and `split_least` at least.  All parts together are at most two
-// for every slot, they come first in the order, and their fp32 sums go to slot = workgroup number; a second kernel adds them
-// in order.
+// Heavy tiles are split: one long prompt's last tile sees all its keys, and alone can take longer than the average workgroup
+// slot has work.  Where it is 1.9 S, S the mean work of the chip's kPackedSlots workgroups and `split_least` at least, tiles of
+// L > S units are cut into ceil(L / S) parts of equal length (2 heads of 128 over one, 16384 tokens: 248 -> 180 us; 4 heads,
+// 12000: 207 -> 178; at 1.3 S, 12 heads, 8192 tokens, parts and their sums cost what they give: 215 -> 231, as a workgroup
+// that has its CU alone runs 1.7 times as fast).  Parts and whole tiles stand in one order, by their work, so the
+// launch's last round is made of light ones; as no part has less than half of S, all parts are among the first 2 kPackedSlots
+// workgroups (and some, as lengths are whole).  A part's fp32 sums go to slot = workgroup number; a second kernel adds them.
 constexpr int kPackedSlots = 512;
-constexpr int kPackedParts = 2 * kPackedSlots;
+constexpr int kPackedParts = 2 * kPackedSlots + 128;
 struct PackedSplit {
-  int S;
+  int S, most;   // units a part has at most; parts a tile has at most
   __device__ __forceinline__ int parts(int L) const { return L > S ? (L + S - 1) / S : 1; }
-  // parts of one tile each of the levels 1 .. x
-  __device__ __forceinline__ int upto(int x) const {
-    if (x <= S) return max(x, 0);
-    const int q = x / S, r = x - q * S;
-    return S * (q * (q + 1) / 2) + r * (q + 1);
+  // a sequence's tiles of P parts with more than x units each
+  __device__ __forceinline__ int above(const PackedTiles& t, int P, int x) const {
+    return x < S ? packed_count(t, max((P - 1) * S, P * x) + 1) - packed_count(t, P * S + 1) : 0;
   }
-  // parts of a sequence's tiles of at least the work `level`
+  // parts of a sequence's tiles that have at least the work `level`
   __device__ __forceinline__ int count(const PackedTiles& t, int level) const {
-    const int n_cap = min(max(t.top - t.cap + 1, 0), t.tiles);   // tiles of work `cap`; the others' falls by one
-    const int from = max(level, max(t.top - t.tiles + 1, 1)), most = min(t.cap - 1, t.top);
-    int c = max(level, 1) <= t.cap ? n_cap * parts(t.cap) : 0;
-    if (most >= from) c += upto(most) - upto(from - 1);
+    int c = 0;
+    for (int P = 1; P <= most; ++P) c += P * above(t, P, max(level, 1) - 1);
     if (level <= 0) c += t.tiles - packed_count(t, 1);   // tiles without work
     return c;
   }
@@ -145,13 +141,21 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
   // (up to 64 sequences: one a lane, in registers)
   const PackedSeq mine = lane < p.n ? seq(lane) : PackedSeq{0, 0, 0, 0};
   const PackedTiles first = packed_tiles<KEYS>(p, mine);
-  PackedSplit split{1 << 28};
+  int best = first.tiles > 0 ? min(first.top, first.cap) : 0;
+  float work = packed_work(first);
+  for (int s = lane + 64; s < p.n; s += 64) {
+    const PackedTiles t = packed_tiles<KEYS>(p, seq(s));
+    best = max(best, t.tiles > 0 ? min(t.top, t.cap) : 0);
+    work += packed_work(t);
+  }
+  best = wave_max_i32(best);
+  PackedSplit split{max(best, 1), 1};
   if (p.split_least > 0) {
-    float work = packed_work(first);
-    for (int s = lane + 64; s < p.n; s += 64) work += packed_work(packed_tiles<KEYS>(p, seq(s)));
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) work += __shfl_xor(work, m);
-    split.S = max(__builtin_amdgcn_readfirstlane((int)ceilf(work * (float)heads * (1.001f / kPackedSlots))), p.split_least);
+    const float mean = work * (float)heads * (1.001f / kPackedSlots);
+    const int S = max(__builtin_amdgcn_readfirstlane((int)ceilf(fminf(mean, 1.0e9f))), p.split_least);
+    if (10 * best >= 19 * S) split = PackedSplit{S, (best + S - 1) / S};
   }
   auto total = [&](int level) __attribute__((always_inline)) {
     int c = split.count(first, level);
@@ -167,33 +171,37 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
   r.parts = 1;
   r.which = idx - all;
   if (idx < all) {
-    int best = first.tiles > 0 ? min(first.top, first.cap) : 0;
-    for (int s = lane + 64; s < p.n; s += 64) {
-      const PackedTiles t = packed_tiles<KEYS>(p, seq(s));
-      best = max(best, t.tiles > 0 ? min(t.top, t.cap) : 0);
-    }
-    int lo = 0, hi = wave_max_i32(best) + 1;   // total(lo) > idx >= total(hi) = 0
+    int lo = 0, hi = min(split.S, best) + 1;   // total(lo) > idx >= total(hi) = 0
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (total(mid) > idx) lo = mid;
       else hi = mid;
     }
     int left = idx - total(lo + 1);
-    const int P = split.parts(lo);
     for (int s0 = 0; s0 < p.n; s0 += 64) {
       const PackedSeq q = s0 == 0 ? mine : s0 + lane < p.n ? seq(s0 + lane) : PackedSeq{0, 0, 0, 0};
       const PackedTiles t = packed_tiles<KEYS>(p, q);
-      const int before = packed_count(t, lo + 1), here = (packed_count(t, lo) - before) * P;
+      const int here = split.count(t, lo) - split.count(t, lo + 1);
       const int upto = wave_scan_i32(here), sum = __builtin_amdgcn_readlane(upto, 63);
       if (left < sum) {
         const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > left));
-        const int in = left - (__builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(here, who));
-        const int u = __builtin_amdgcn_readlane(before, who) + in / P;
+        left -= __builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(here, who);
+        const PackedTiles it{__builtin_amdgcn_readlane(t.tiles, who), __builtin_amdgcn_readlane(t.top, who),
+                             __builtin_amdgcn_readlane(t.cap, who)};
+        int P = 1, u = packed_count(it, 1) + left;   // (a tile without work)
+        if (lo > 0) {
+          for (; P < split.most; ++P) {
+            const int of_p = P * (split.above(it, P, lo - 1) - split.above(it, P, lo));
+            if (left < of_p) break;
+            left -= of_p;
+          }
+          u = packed_count(it, min(P * split.S, P * lo) + 1) + left / P;
+        }
         r.s = PackedSeq{__builtin_amdgcn_readlane(q.qb, who), __builtin_amdgcn_readlane(q.nq, who),
                         __builtin_amdgcn_readlane(q.kb, who), __builtin_amdgcn_readlane(q.nk, who)};
-        r.tile = KEYS || !p.causal ? u : __builtin_amdgcn_readlane(t.tiles, who) - 1 - u;
+        r.tile = KEYS || !p.causal ? u : it.tiles - 1 - u;
         r.parts = P;
-        r.part = in % P;
+        r.part = lo > 0 ? left % P : 0;
         break;
       }
       left -= sum;
@@ -309,11 +317,12 @@ inline int64_t packed_grid(int rows, int n, int heads, bool split) {
   const int64_t tiles = (int64_t)(rows + kPackedTile - 1) / kPackedTile + n;
   return (tiles + (split ? (kPackedParts + heads - 1) / heads : 0)) * heads;
 }
-// Whether tiles are split: long sequences on average, some of them with more than kPackedSplit units.  (Offsets are on the
-// GPU: the host sees the sums alone.  In a batch of short prompts, 12 of 40 to 2900 tokens, parts and their sums cost more
-// than the balance gives: 65.8 -> 82 us.)
+// Whether tiles may be split (`others`: rows of the other side): sequences of 2048 on average, one of 46 units among them, and
+// few enough workgroups that one can have 1.9 times the mean.  Offsets are on the GPU: the host sees sums alone.
 constexpr int kPackedSplit = 24;
-inline bool packed_splits(int64_t others, int n) { return others > kPackedSplit * kPackedTile && others >= 2048ll * n; }
+inline bool packed_splits(int64_t others, int n, int64_t grid) {
+  return others > 45 * kPackedTile && others >= 2048ll * n && grid <= 960;
+}
 
 int packed_fwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);
 int packed_bwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);

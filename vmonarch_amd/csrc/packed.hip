@@ -50,17 +50,18 @@ static int packed_prepare(const vmo_packed_args* a, bool bwd, const char* what, 
 // Workspaces: the parts of split tiles (the forward's with their m and l, the backward's of dq, then of dk and dv), and
 // before them the backward's -delta.  Some slots more than kPackedParts: parts come in whole heads.
 static int64_t part_floats(int d, int heads) { return (int64_t)(kPackedParts + heads) * kPackedTile * d; }
+static bool splits_q(const vmo_packed_args* a) { return packed_splits(a->tk, a->n, packed_grid(a->tq, a->n, a->heads, false)); }
 static int64_t fwd_layout(const vmo_packed_args* a) {
-  return packed_splits(a->tk, a->n) ? (part_floats(a->d, a->heads) + part_floats(2, a->heads)) * 4 : 0;
+  return splits_q(a) ? (part_floats(a->d, a->heads) + part_floats(2, a->heads)) * 4 : 0;
 }
 struct BwdLayout { int64_t delta, kv, bytes; int splits; };   // floats of -delta and of dk's parts
 static BwdLayout bwd_layout(const vmo_packed_args* a) {
   BwdLayout l;
   l.delta = ((int64_t)a->heads * a->tq + 63) / 64 * 64;
   l.splits = packed_bwd_splits(a->tk, a->kv_heads, a->heads / a->kv_heads);
-  const int64_t q = packed_splits(a->tk, a->n) ? part_floats(a->d, a->heads) : 0;
+  const int64_t q = splits_q(a) ? part_floats(a->d, a->heads) : 0;
   l.kv = l.splits > 1 ? (int64_t)l.splits * a->kv_heads * a->tk * a->d
-         : packed_splits(a->tq, a->n) ? part_floats(a->d, a->kv_heads) : 0;
+         : packed_splits(a->tq, a->n, packed_grid(a->tk, a->n, a->kv_heads, false)) ? part_floats(a->d, a->kv_heads) : 0;
   l.bytes = (l.delta + (q > 2 * l.kv ? q : 2 * l.kv)) * 4;
   return l;
 }
@@ -86,7 +87,7 @@ extern "C" int vmo_packed_fwd(const vmo_packed_args* a, void* stream) {
   if (rc != VMO_OK || a->tq == 0) return rc;
   rc = workspace_check(a, fwd_layout(a), "packed_fwd");
   if (rc != VMO_OK) return rc;
-  if (packed_splits(a->tk, a->n)) {
+  if (splits_q(a)) {
     p.split_least = kPackedSplit;
     p.part = (float*)a->workspace;
     p.part2 = p.part + part_floats(a->d, a->heads);

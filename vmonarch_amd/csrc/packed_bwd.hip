@@ -486,7 +486,7 @@ static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   };
   int rc = VMO_OK;
   if (p.tq > 0) {
-    p.split_least = packed_splits(p.tk, p.n) ? kPackedSplit : 0;
+    p.split_least = packed_splits(p.tk, p.n, packed_grid(p.tq, p.n, p.heads, false)) ? kPackedSplit : 0;
     const int64_t grid = packed_grid(p.tq, p.n, p.heads, p.split_least > 0);
     hipLaunchKernelGGL((packed_bwd_dq_kernel<F16, D>), dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_Q, s, p);
     rc = launch_status("packed_bwd_dq");
@@ -498,7 +498,7 @@ static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   if (LDS_KV > 65536 &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_KV) != hipSuccess)
     return set_error(VMO_ERR_LAUNCH, "packed_bwd: cannot raise the LDS limit to %d bytes", LDS_KV);
-  p.split_least = p.splits == 1 && packed_splits(p.tq, p.n) ? kPackedSplit : 0;
+  p.split_least = p.splits == 1 && packed_splits(p.tq, p.n, packed_grid(p.tk, p.n, p.kv_heads, false)) ? kPackedSplit : 0;
   const int64_t grid = packed_grid(p.tk, p.n, p.kv_heads * p.splits, p.split_least > 0);
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_KV, s, p);
   rc = launch_status("packed_bwd_dkdv");

@@ -17,7 +17,6 @@
 //  * where the launch is small, eight waves share the 128 queries: two groups of four take every other stage, each with a
 //    ring of its own, and the second's sums join the first's in LDS (G = 2).
 // The row sums add the fp32 p; p is rounded to the 16-bit type as the operand of P V, o once at the end.
-#include <stdlib.h>
 #include "packed.h"
 
 namespace vmo {
@@ -377,10 +376,10 @@ template <bool F16, int D>
 static int dispatch_packed_fwd(PackedParams p, hipStream_t s) {
   const int64_t grid = packed_grid(p.tq, p.n, p.heads, p.split_least > 0);
   // Two key groups halve the longest workgroup's time, which is the launch's where the chip holds all of them at once (one
-  // prompt of 2048 tokens, 12 heads of 128: 38.8 -> 34.7 us; of 4096, 80.2 -> 65.7, where splitting tiles gives @@); with
-  // more workgroups, the barriers that eight waves share cost (8192 tokens 214.6 -> 224.4 us), and for short prompts the
-  // join does (four of up to 200 tokens, 64 wide: 8.9 -> 9.6 us).
-  const bool two = getenv("PG") ? atoi(getenv("PG")) == 2 : p.split_least == 0 && grid <= 512 && p.tk >= 768ll * p.n;
+  // prompt of 4096 tokens, 12 heads of 128: 80.2 -> 65.7 us, of 2048: 38.8 -> 34.7); with more workgroups, the barriers that
+  // eight waves share cost (8192 tokens 214.6 -> 224.4 us), for short prompts the join does (four of up to 200 tokens, 64
+  // wide: 8.9 -> 9.6 us), and parts of tiles do more for the longest (2 heads, 16384 tokens: 204 us so, 180 in parts).
+  const bool two = p.split_least == 0 && grid <= 512 && p.tk >= 768ll * p.n;
   const int rc = two ? launch_packed_fwd<F16, D, 2>(p, grid, s) : launch_packed_fwd<F16, D, 1>(p, grid, s);
   if (rc != VMO_OK || p.split_least == 0) return rc;
   const int64_t slots = (kPackedParts + p.heads - 1) / p.heads * p.heads;
