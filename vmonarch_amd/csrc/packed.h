@@ -27,6 +27,7 @@ struct PackedParams {
   float* neg_delta;                        // (heads, tq): -rowsum(o dO), from the dq kernel to the dk / dv one
   float *part, *part2;                     // parts of split tiles: (slots, 128, D) fp32 sums; the forward's m and l (.., 2), or dv's
                                            // (splits > 1: dk's and dv's (splits, kv_heads, tk, D))
+  i32x4* records;                          // of the first kPackedParts workgroups: first row, rows, part and parts of its tile
   int splits;                              // dk / dv: workgroups that share a key tile, each with group / splits of the heads
   int split_least;                         // tiles of up to so many units are never split (0: no tile is)
   float c, sm_scale;                       // c = sm_scale log2 e
@@ -82,13 +83,15 @@ __device__ __forceinline__ int packed_count(const PackedTiles& t, int level) {
   return level <= t.cap ? min(max(t.top - level + 1, 0), t.tiles) : 0;
 }
 
-// Heavy tiles are split: one long prompt's last tile sees all its keys, and alone can take longer than the average workgroup
-// slot has work.  Where it is 1.9 S, S the mean work of the chip's kPackedSlots workgroups and `split_least` at least, tiles of
-// L > S units are cut into ceil(L / S) parts of equal length (2 heads of 128 over one, 16384 tokens: 248 -> 180 us; 4 heads,
-// 12000: 207 -> 178; at 1.3 S, 12 heads, 8192 tokens, parts and their sums cost what they give: 215 -> 231, as a workgroup
-// that has its CU alone runs 1.7 times as fast).  Parts and whole tiles stand in one order, by their work, so the
-// launch's last round is made of light ones; as no part has less than half of S, all parts are among the first 2 kPackedSlots
-// workgroups (and some, as lengths are whole).  A part's fp32 sums go to slot = workgroup number; a second kernel adds them.
+// Heavy tiles are split: one long prompt's last tile sees all its keys, and alone can take longer than the whole launch's mean
+// work.  S is 1.75 times the mean of the chip's kPackedSlots workgroups -- one that has its CU alone runs about that much
+// faster than two that share it, so up to S a tile is no later than the rest -- and `split_least` at least; where the
+// heaviest tile has 1.25 S, those of L > S units are cut into ceil(L / S) parts of equal length.  One prompt of 16384 tokens,
+// 2 heads of 128 over one: 248 -> 168 us; of 8192, 4 heads: 129 -> 97; 4 prompts of 20 to 5000, 4 heads: 85 -> 59; with S the
+// mean itself the parts' own cost shows (8192 tokens, 12 heads: 215 -> 231), and eight waves of two key groups instead, which
+// halve every tile's time, did less (176 and 99 -> 218 and 116).  Parts and whole tiles stand in one order, by their work, so
+// the launch's last round is made of light ones; as no part has less than half of S, all parts are among the first
+// 2 kPackedSlots / 1.75 workgroups.  A part's fp32 sums go to slot = workgroup number; a second kernel adds them.
 constexpr int kPackedSlots = 512;
 constexpr int kPackedParts = 2 * kPackedSlots + 128;
 struct PackedSplit {
@@ -154,8 +157,8 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) work += __shfl_xor(work, m);
     const float mean = work * (float)heads * (1.001f / kPackedSlots);
-    const int S = max(__builtin_amdgcn_readfirstlane((int)ceilf(fminf(mean, 1.0e9f))), p.split_least);
-    if (10 * best >= 19 * S) split = PackedSplit{S, (best + S - 1) / S};
+    const int S = max(__builtin_amdgcn_readfirstlane((int)ceilf(fminf(1.75f * mean, 1.0e9f))), p.split_least);
+    if (4 * best >= 5 * S) split = PackedSplit{S, (best + S - 1) / S};
   }
   auto total = [&](int level) __attribute__((always_inline)) {
     int c = split.count(first, level);
@@ -209,6 +212,15 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
   }
   __syncthreads();   // every wave has read the sequences
   return r;
+}
+
+// What the adding kernel has to know of this workgroup's tile (rows of the side that the tile is of).
+template <bool KEYS>
+__device__ __forceinline__ void packed_record(const PackedParams& p, const PackedTile& w) {
+  if (p.split_least > 0 && blockIdx.x < kPackedParts && threadIdx.x == 0) {
+    const int first = w.tile * kPackedTile, rows = min(kPackedTile, (KEYS ? w.s.nk : w.s.nq) - first);
+    p.records[blockIdx.x] = i32x4{(KEYS ? w.s.kb : w.s.qb) + first, rows, w.part, w.tile < 0 ? 1 : w.parts};
+  }
 }
 
 // Zeros for the rows outside every sequence, 128-row pieces dealt to the spare workgroups (there is one at least
@@ -317,12 +329,10 @@ inline int64_t packed_grid(int rows, int n, int heads, bool split) {
   const int64_t tiles = (int64_t)(rows + kPackedTile - 1) / kPackedTile + n;
   return (tiles + (split ? (kPackedParts + heads - 1) / heads : 0)) * heads;
 }
-// Whether tiles may be split (`others`: rows of the other side): sequences of 2048 on average, one of 46 units among them, and
-// few enough workgroups that one can have 1.9 times the mean.  Offsets are on the GPU: the host sees sums alone.
-constexpr int kPackedSplit = 24;
-inline bool packed_splits(int64_t others, int n, int64_t grid) {
-  return others > 45 * kPackedTile && others >= 2048ll * n && grid <= 960;
-}
+// Whether tiles may be split (`others`: rows of the other side, in all: offsets are on the GPU): the second kernel's launch,
+// 3 us where it finds nothing to add, is spared short batches.
+constexpr int kPackedSplit = 5;
+inline bool packed_splits(int64_t others) { return others > 1536; }
 
 int packed_fwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);
 int packed_bwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);

@@ -47,22 +47,22 @@ static int packed_prepare(const vmo_packed_args* a, bool bwd, const char* what, 
   return VMO_OK;
 }
 
-// Workspaces: the parts of split tiles (the forward's with their m and l, the backward's of dq, then of dk and dv), and
-// before them the backward's -delta.  Some slots more than kPackedParts: parts come in whole heads.
-static int64_t part_floats(int d, int heads) { return (int64_t)(kPackedParts + heads) * kPackedTile * d; }
-static bool splits_q(const vmo_packed_args* a) { return packed_splits(a->tk, a->n, packed_grid(a->tq, a->n, a->heads, false)); }
+// Workspaces: the records of split tiles and their parts (the forward's with their m and l, the backward's of dq, then of dk
+// and dv), between them the backward's -delta.
+static int64_t part_floats(int d) { return (int64_t)kPackedParts * kPackedTile * d; }
+constexpr int64_t kRecordFloats = (int64_t)kPackedParts * 4;
 static int64_t fwd_layout(const vmo_packed_args* a) {
-  return splits_q(a) ? (part_floats(a->d, a->heads) + part_floats(2, a->heads)) * 4 : 0;
+  return packed_splits(a->tk) ? (kRecordFloats + part_floats(a->d) + part_floats(2)) * 4 : 0;
 }
 struct BwdLayout { int64_t delta, kv, bytes; int splits; };   // floats of -delta and of dk's parts
 static BwdLayout bwd_layout(const vmo_packed_args* a) {
   BwdLayout l;
   l.delta = ((int64_t)a->heads * a->tq + 63) / 64 * 64;
   l.splits = packed_bwd_splits(a->tk, a->kv_heads, a->heads / a->kv_heads);
-  const int64_t q = splits_q(a) ? part_floats(a->d, a->heads) : 0;
+  const int64_t q = packed_splits(a->tk) ? part_floats(a->d) : 0;
   l.kv = l.splits > 1 ? (int64_t)l.splits * a->kv_heads * a->tk * a->d
-         : packed_splits(a->tq, a->n, packed_grid(a->tk, a->n, a->kv_heads, false)) ? part_floats(a->d, a->kv_heads) : 0;
-  l.bytes = (l.delta + (q > 2 * l.kv ? q : 2 * l.kv)) * 4;
+         : packed_splits(a->tq) ? part_floats(a->d) : 0;
+  l.bytes = (kRecordFloats + l.delta + (q > 2 * l.kv ? q : 2 * l.kv)) * 4;
   return l;
 }
 static bool sizes_ok(const vmo_packed_args* a) {
@@ -87,10 +87,11 @@ extern "C" int vmo_packed_fwd(const vmo_packed_args* a, void* stream) {
   if (rc != VMO_OK || a->tq == 0) return rc;
   rc = workspace_check(a, fwd_layout(a), "packed_fwd");
   if (rc != VMO_OK) return rc;
-  if (splits_q(a)) {
+  if (packed_splits(a->tk)) {
     p.split_least = kPackedSplit;
-    p.part = (float*)a->workspace;
-    p.part2 = p.part + part_floats(a->d, a->heads);
+    p.records = (i32x4*)a->workspace;
+    p.part = (float*)a->workspace + kRecordFloats;
+    p.part2 = p.part + part_floats(a->d);
   }
   return packed_fwd_launch(p, a->dtype == VMO_DTYPE_F16, a->d, (hipStream_t)stream);
 }
@@ -109,7 +110,8 @@ extern "C" int vmo_packed_bwd(const vmo_packed_args* a, void* stream) {
   rc = workspace_check(a, l.bytes, "packed_bwd");
   if (rc != VMO_OK) return rc;
   p.splits = l.splits;
-  p.neg_delta = (float*)a->workspace;
+  p.records = (i32x4*)a->workspace;
+  p.neg_delta = (float*)a->workspace + kRecordFloats;
   p.part = p.neg_delta + l.delta;
   p.part2 = p.part + l.kv;
   return packed_bwd_launch(p, a->dtype == VMO_DTYPE_F16, a->d, (hipStream_t)stream);

@@ -52,6 +52,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
 
   const int head = uni(packed_head((int)blockIdx.x % p.heads, p.heads));
   const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, p.heads, (VMO_LDS int*)smem);
+  packed_record<false>(p, w);
   if (w.tile < 0) {
     packed_zero_rest<T, D>((T*)p.dq + head * p.dq_sh, p.dq_sn, p.q_off, p.n, p.tq, w.which, w.spare);
     return;
@@ -205,6 +206,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   const int hs = uni(packed_head((int)blockIdx.x % shares, shares));
   const int kvh = hs / p.splits, split = hs % p.splits;
   const PackedTile w = packed_locate<true>(p, (int)blockIdx.x / shares, (int)gridDim.x / shares, shares, (VMO_LDS int*)smem);
+  packed_record<true>(p, w);
   if (w.tile < 0) {
     if (p.splits == 1) {
       packed_zero_rest<T, D>((T*)p.dk + kvh * p.dk_sh, p.dk_sn, p.k_off, p.n, p.tk, w.which, w.spare);
@@ -401,16 +403,15 @@ __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams p) {
   using T = typename Elem<F16>::T;
   using V4 = typename Elem<F16>::V4;
   constexpr int TPR = D / 4;
-  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
-  const int heads = KEYS ? p.kv_heads : p.heads, head = packed_head((int)blockIdx.x % heads, heads);
-  const PackedTile w = packed_locate<KEYS>(p, (int)blockIdx.x / heads, 1 << 20, heads, (VMO_LDS int*)(VMO_LDS char*)smem_raw);
-  if (w.tile < 0 || w.parts == 1) return;
-  const int rows = min(kPackedTile, (KEYS ? w.s.nk : w.s.nq) - w.tile * kPackedTile), d4 = (threadIdx.x % TPR) * 4;
-  const int64_t slot0 = (int)blockIdx.x - w.part * heads;
-  for (int r = w.part * rows / w.parts + threadIdx.x / TPR; r < (w.part + 1) * rows / w.parts; r += 256 / TPR) {
+  const i32x4 rec = p.records[blockIdx.x];   // first row, rows, part, parts
+  if (rec[3] <= 1) return;
+  const int heads = KEYS ? p.kv_heads : p.heads, head = packed_head((int)blockIdx.x % heads, heads), parts = rec[3];
+  const int d4 = (threadIdx.x % TPR) * 4;
+  const int64_t slot0 = (int)blockIdx.x - rec[2] * heads;
+  for (int r = rec[2] * rec[1] / parts + threadIdx.x / TPR; r < (rec[2] + 1) * rec[1] / parts; r += 256 / TPR) {
     f32x4 a = f32x4{}, b = f32x4{};
 #pragma unroll 4
-    for (int i = 0; i < w.parts; ++i) {
+    for (int i = 0; i < parts; ++i) {
       const int64_t at = ((slot0 + i * heads) * kPackedTile + r) * D + d4;
       a += *(const f32x4*)(p.part + at);
       if constexpr (KEYS) b += *(const f32x4*)(p.part2 + at);
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams p) {
       x[e] = to_elem<T>(a[e]);
       y[e] = to_elem<T>(b[e]);
     }
-    const int64_t tok = (KEYS ? w.s.kb : w.s.qb) + w.tile * kPackedTile + r;
+    const int64_t tok = rec[0] + r;
     if constexpr (KEYS) {
       *(V4*)((T*)p.dk + (int64_t)head * p.dk_sh + tok * p.dk_sn + d4) = x;
       *(V4*)((T*)p.dv + (int64_t)head * p.dv_sh + tok * p.dv_sn + d4) = y;
@@ -479,18 +480,17 @@ template <bool F16, int D>
 static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   constexpr int LDS_Q = packed_dq_lds<D>(), LDS_KV = packed_kv_lds<D>();
   static_assert(LDS_Q <= 65536 && LDS_KV <= 80 * 1024, "two workgroups a CU");
-  auto join = [&](auto kern, int heads) {
-    const int64_t slots = (kPackedParts + heads - 1) / heads * heads;
-    hipLaunchKernelGGL(kern, dim3((unsigned)slots), dim3(256), kPackedSeqBytes * kPackedMaxSeqs, s, p);
+  auto join = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3(kPackedParts), dim3(256), 0, s, p);
     return launch_status("packed_bwd_join");
   };
   int rc = VMO_OK;
   if (p.tq > 0) {
-    p.split_least = packed_splits(p.tk, p.n, packed_grid(p.tq, p.n, p.heads, false)) ? kPackedSplit : 0;
+    p.split_least = packed_splits(p.tk) ? kPackedSplit : 0;
     const int64_t grid = packed_grid(p.tq, p.n, p.heads, p.split_least > 0);
     hipLaunchKernelGGL((packed_bwd_dq_kernel<F16, D>), dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_Q, s, p);
     rc = launch_status("packed_bwd_dq");
-    if (rc == VMO_OK && p.split_least > 0) rc = join(packed_bwd_join_kernel<F16, D, false>, p.heads);
+    if (rc == VMO_OK && p.split_least > 0) rc = join(packed_bwd_join_kernel<F16, D, false>);
     if (rc != VMO_OK) return rc;
   }
   if (p.tk == 0) return VMO_OK;
@@ -498,12 +498,12 @@ static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   if (LDS_KV > 65536 &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_KV) != hipSuccess)
     return set_error(VMO_ERR_LAUNCH, "packed_bwd: cannot raise the LDS limit to %d bytes", LDS_KV);
-  p.split_least = p.splits == 1 && packed_splits(p.tq, p.n, packed_grid(p.tk, p.n, p.kv_heads, false)) ? kPackedSplit : 0;
+  p.split_least = p.splits == 1 && packed_splits(p.tq) ? kPackedSplit : 0;
   const int64_t grid = packed_grid(p.tk, p.n, p.kv_heads * p.splits, p.split_least > 0);
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_KV, s, p);
   rc = launch_status("packed_bwd_dkdv");
   if (rc != VMO_OK) return rc;
-  if (p.split_least > 0) return join(packed_bwd_join_kernel<F16, D, true>, p.kv_heads);
+  if (p.split_least > 0) return join(packed_bwd_join_kernel<F16, D, true>);
   if (p.splits == 1) return VMO_OK;
   const int64_t threads = (int64_t)p.kv_heads * p.tk * (D / 4);
   hipLaunchKernelGGL((packed_bwd_sum_kernel<F16, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);

@@ -14,8 +14,7 @@
 //    costs 16 vector operations a block more).  The loop notes that a limit was passed, and then the workgroup runs its
 //    keys again with the test; rows that pass no limit have the same bits both ways.
 //  * workgroups take the heaviest tile first (packed_locate).
-//  * where the launch is small, eight waves share the 128 queries: two groups of four take every other stage, each with a
-//    ring of its own, and the second's sums join the first's in LDS (G = 2).
+//  * tiles whose keys would take longer than the rest of the launch are cut into parts, whose sums packed_fwd_join adds.
 // The row sums add the fp32 p; p is rounded to the 16-bit type as the operand of P V, o once at the end.
 #include "packed.h"
 
@@ -26,14 +25,14 @@ template <bool F16> constexpr float kSumMost = F16 ? 32768.f : 1099511627776.f;
 constexpr float kNoMax = -3.0e38f;    // m of a row that has seen no key
 
 template <int D> constexpr int packed_stage_bytes() { return kFwdBN * D * 2 * 2; }
-template <int D, int G> constexpr int packed_fwd_lds() {
-  constexpr int ring = G * fwd_slots(packed_stage_bytes<D>()) * packed_stage_bytes<D>();
+template <int D> constexpr int packed_fwd_lds() {
+  constexpr int ring = fwd_slots(packed_stage_bytes<D>()) * packed_stage_bytes<D>();
   constexpr int least = kPackedWaves * kEpiPatchBytes > kPackedSeqBytes * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : kPackedSeqBytes * kPackedMaxSeqs;
   return ring > least ? ring : least;
 }
 
-template <bool F16, int D, int G>
-__global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kernel(PackedParams p) {
+template <bool F16, int D>
+__global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(PackedParams p) {
   using E = Elem<F16>;
   using T = typename E::T;
   using V8 = typename E::V8;
@@ -47,16 +46,14 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
 
   const int head = uni(packed_head((int)blockIdx.x % p.heads, p.heads));
   const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, p.heads, (VMO_LDS int*)smem);
+  packed_record<false>(p, w);
   if (w.tile < 0) {
     if (p.zero_rest)
       packed_zero_rest<T, D>((T*)p.out + head * p.o_sh, p.o_sn, p.q_off, p.n, p.tq, w.which, w.spare);
     return;
   }
   const int nq = uni(w.s.nq), nk = uni(w.s.nk), qb = uni(w.s.qb), kb = uni(w.s.kb);
-  const int tid = threadIdx.x, wave = uni((tid >> 6) % kPackedWaves), grp = G > 1 ? uni((tid >> 6) / kPackedWaves) : 0;
-  const int lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
-  VMO_LDS char* ring = smem + grp * NSLOT * STAGE;   // the key group's own
-  const uint32_t ring_u32 = (uint32_t)(uintptr_t)ring;
+  const int tid = threadIdx.x, wave = uni(tid >> 6), lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int q0 = uni(w.tile) * kPackedTile + wave * 32;   // the wave's first row of the sequence
   const bool live = q0 < nq;
   // keys that row i sees: the first sees(i) of the sequence
@@ -65,28 +62,27 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
   const int row = min(q0 + l32, nq - 1);
   const int lim = keys_of(row);
   const int lo = uni(keys_of(min(q0, nq - 1))), hi = uni(keys_of(min(q0 + 31, nq - 1)));   // least and most of the wave
-  // the part's stages, from `begin` on, and those of them that the key group takes
+  // the part's stages: n_tiles from `begin` on
   const int stages = uni((keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 1, nq - 1)) + kFwdBN - 1) / kFwdBN);
-  const int parts = uni(w.parts), begin = uni((int)((int64_t)w.part * stages / parts)) + grp;
-  const int all_tiles = uni((int)((int64_t)(w.part + 1) * stages / parts)) + grp - begin;
-  const int n_tiles = G > 1 ? (all_tiles - grp + G - 1) / G : all_tiles, steps = (all_tiles + G - 1) / G;
+  const int parts = uni(w.parts), begin = uni((int)((int64_t)w.part * stages / parts));
+  const int n_tiles = uni((int)((int64_t)(w.part + 1) * stages / parts)) - begin;
 
   const T* kbase = (const T*)p.k + (int64_t)(head / p.group) * p.k_sh + (int64_t)kb * p.k_sn;
   const T* vbase = (const T*)p.v + (int64_t)(head / p.group) * p.v_sh + (int64_t)kb * p.v_sn;
   const TileCopy<T, D, kPackedWaves> kcopy(kbase, p.k_sn, wave, lane), vcopy(vbase, p.v_sn, wave, lane);
   auto issue = [&](int t) __attribute__((always_inline)) {
-    uint32_t sb = ring_u32;
+    uint32_t sb = (uint32_t)(uintptr_t)smem;
     asm volatile("" : "+s"(sb));
     const uint32_t st = sb + (uint32_t)((t % NSLOT) * STAGE);
-    kcopy.issue((begin + t * G) * kFwdBN, nk, st);   // (a tile that runs past the sequence repeats its last key: masked)
-    vcopy.issue((begin + t * G) * kFwdBN, nk, st + K_BYTES);
+    kcopy.issue((begin + t) * kFwdBN, nk, st);   // (a tile that runs past the sequence repeats its last key: masked)
+    vcopy.issue((begin + t) * kFwdBN, nk, st + K_BYTES);
   };
 
   auto prime = [&]() __attribute__((always_inline)) {
-    if (n_tiles > 0) issue(0);
+    issue(0);
     if (NSLOT == 3 && n_tiles > 1) issue(1);
   };
-  prime();   // the first copies are under way while the queries come
+  if (n_tiles > 0) prime();   // the first copies are under way while the queries come
   V8 qf[NDS];   // Q^T as the B operand: lane (query l32, half hl) holds features 16 ds + 8 hl + 0..7
   {
     const T* qp = (const T*)p.q + (int64_t)head * p.q_sh + (int64_t)(qb + row) * p.q_sn + hl * 8;
@@ -236,16 +232,16 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
   // Tile t sits in ring slot t % NSLOT; at its top this wave's copies of it have landed (only those of tile t + 1 may be
   // under way), after the barrier every wave's have, and the slot of tile t - 1 is free for tile t + NSLOT - 1.
   constexpr int kSteadyPending = NSLOT == 3 ? DMA_PER_TILE : 0;
-  const int n_full = live ? uni(min(max((lo / kFwdBN - begin + G - 1) / G, 0), n_tiles)) : 0;
+  const int n_full = live ? uni(min(max(lo / kFwdBN - begin, 0), n_tiles)) : 0;
   auto top = [&](int t) __attribute__((always_inline)) {
     if (NSLOT == 3 && t + 1 < n_tiles) tile_sync<kSteadyPending>();
     else tile_sync<0>();
     if (t + NSLOT - 1 < n_tiles) issue(t + NSLOT - 1);
   };
-  auto slot = [&](int t) __attribute__((always_inline)) { return (const VMO_LDS char*)ring + (t % NSLOT) * STAGE; };
+  auto slot = [&](int t) __attribute__((always_inline)) { return (const VMO_LDS char*)smem + (t % NSLOT) * STAGE; };
   // stages that some wave of the workgroup runs untested (the last wave's rows see most)
-  const int untested = uni(max(keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 32, nq - 1)) / kFwdBN - G, 0));
-  for (bool again = false; steps > 0; again = true) {
+  const int untested = uni(max(keys_of(min(uni(w.tile) * kPackedTile + kPackedTile - 32, nq - 1)) / kFwdBN - begin - 1, 0));
+  for (bool again = false; n_tiles > 0; again = true) {
     if (again) prime();
     int t = 0;
     const int tested = again ? n_full : min(1, n_full);   // the first stage sets m
@@ -256,15 +252,15 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
     for (; t + NSLOT <= n_full; t += NSLOT)   // (t = 1, 1 + NSLOT, ..: slots at compile-time offsets)
       static_for<0, NSLOT>([&](auto i) __attribute__((always_inline)) {
         top(t + decltype(i)::value);
-        full_stage((const VMO_LDS char*)ring + ((1 + decltype(i)::value) % NSLOT) * STAGE, std::false_type{});
+        full_stage((const VMO_LDS char*)smem + ((1 + decltype(i)::value) % NSLOT) * STAGE, std::false_type{});
       });
     for (; t < n_full; ++t) {
       top(t);
       full_stage(slot(t), std::false_type{});
     }
-    for (; t < steps; ++t) {
+    for (; t < n_tiles; ++t) {
       top(t);
-      const int key0 = (begin + t * G) * kFwdBN;
+      const int key0 = (begin + t) * kFwdBN;
       if (live && key0 < hi) masked_stage(slot(t), key0);
     }
     __syncthreads();   // the ring is free
@@ -272,11 +268,11 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
     // whether any row of the workgroup passed the limit untested: a word a wave in the ring
     VMO_LDS int* words = (VMO_LDS int*)smem;
     const bool mine = __builtin_amdgcn_ballot_w64(passed) != 0;
-    if (lane == 0) words[grp * kPackedWaves + wave] = mine;
+    if (lane == 0) words[wave] = mine;
     __syncthreads();
     int any = 0;
 #pragma unroll
-    for (int i = 0; i < G * kPackedWaves; ++i) any |= words[i];
+    for (int i = 0; i < kPackedWaves; ++i) any |= words[i];
     __syncthreads();
     if (!any) break;
     m_run = kNoMax;
@@ -284,33 +280,10 @@ __global__ __launch_bounds__(64 * kPackedWaves * G, 2 / G) void packed_fwd_kerne
 #pragma unroll
     for (int a = 0; a < NA; ++a) acc[a] = f32x16{};
   }
-  float l_tot = wave_sum32(l_run);
-  if constexpr (G > 1) {   // the second group's sums join the first's, through LDS (a lane reads what its fellow wrote)
-    static_assert(G == 2 && kPackedWaves * (NA * 16 + 2) * 256 <= G * NSLOT * STAGE, "two groups");
-    VMO_LDS float* box = (VMO_LDS float*)(smem + wave * (NA * 16 + 2) * 256) + lane;
-    if (grp == 1) {
-      box[0] = m_run;
-      box[64] = l_tot;
-#pragma unroll
-      for (int a = 0; a < NA; ++a)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) box[(2 + a * 16 + r) * 64] = acc[a][r];
-    }
-    __syncthreads();
-    if (grp == 1) return;
-    const float m1 = box[0], m = fmaxf(m_run, m1), f0 = fast_exp2(m_run - m), f1 = fast_exp2(m1 - m);
-    l_tot = fmaf(l_tot, f0, box[64] * f1);
-    m_run = m;
-#pragma unroll
-    for (int a = 0; a < NA; ++a)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[a][r] = fmaf(acc[a][r], f0, box[(2 + a * 16 + r) * 64] * f1);
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-    // (each wave's row patch lies in its own box)
-  }
   if (!live) return;
+  const float l_tot = wave_sum32(l_run);
   const int nrows = min(32, nq - q0);
-  VMO_LDS float* patch = (VMO_LDS float*)(smem + wave * (G > 1 ? (NA * 16 + 2) * 256 : kEpiPatchBytes));
+  VMO_LDS float* patch = (VMO_LDS float*)(smem + wave * kEpiPatchBytes);
   if (parts > 1) {
     const int64_t at = (int64_t)blockIdx.x * kPackedTile + wave * 32;
     store_acc_rows<F16>(patch, acc, NA, 1.f, kGradStoreF32, (char*)(p.part + at * D), D * 4, nrows, lane);
@@ -332,17 +305,15 @@ template <bool F16, int D>
 __global__ __launch_bounds__(256) void packed_fwd_join_kernel(PackedParams p) {
   using T = typename Elem<F16>::T;
   constexpr int TPR = D / 4;
-  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
-  const int head = packed_head((int)blockIdx.x % p.heads, p.heads);
-  const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, 1 << 20, p.heads, (VMO_LDS int*)(VMO_LDS char*)smem_raw);
-  if (w.tile < 0 || w.parts == 1) return;
-  const int rows = min(kPackedTile, w.s.nq - w.tile * kPackedTile), d4 = (threadIdx.x % TPR) * 4;
-  const int slot0 = (int)blockIdx.x - w.part * p.heads;
-  for (int r = w.part * rows / w.parts + threadIdx.x / TPR; r < (w.part + 1) * rows / w.parts; r += 256 / TPR) {
+  const i32x4 rec = p.records[blockIdx.x];   // first row, rows, part, parts
+  if (rec[3] <= 1) return;
+  const int head = packed_head((int)blockIdx.x % p.heads, p.heads), d4 = (threadIdx.x % TPR) * 4, parts = rec[3];
+  const int slot0 = (int)blockIdx.x - rec[2] * p.heads;
+  for (int r = rec[2] * rec[1] / parts + threadIdx.x / TPR; r < (rec[2] + 1) * rec[1] / parts; r += 256 / TPR) {
     float m = kNoMax, l = 0.f;
     f32x4 acc = f32x4{};
 #pragma unroll 4
-    for (int i = 0; i < w.parts; ++i) {
+    for (int i = 0; i < parts; ++i) {
       const int64_t at = (int64_t)(slot0 + i * p.heads) * kPackedTile + r;
       const float pm = p.part2[2 * at], pl = p.part2[2 * at + 1];
       const f32x4 y = *(const f32x4*)(p.part + at * D + d4);
@@ -356,40 +327,27 @@ __global__ __launch_bounds__(256) void packed_fwd_join_kernel(PackedParams p) {
     typename Elem<F16>::V4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = to_elem<T>(acc[e] * inv);
-    const int64_t tok = w.s.qb + w.tile * kPackedTile + r;
+    const int64_t tok = rec[0] + r;
     *(typename Elem<F16>::V4*)((T*)p.out + (int64_t)head * p.o_sh + tok * p.o_sn + d4) = y;
     if (p.lse && d4 == 0) p.lse[(int64_t)head * p.st_sh + tok] = l == 0.f ? 0.f : m + fast_log2(l);
   }
 }
 
-template <bool F16, int D, int G>
-static int launch_packed_fwd(const PackedParams& p, int64_t grid, hipStream_t s) {
-  constexpr int LDS = packed_fwd_lds<D, G>();
-  auto kern = packed_fwd_kernel<F16, D, G>;
-  if (LDS > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
-    return set_error(VMO_ERR_LAUNCH, "packed_fwd: cannot raise the LDS limit to %d bytes", LDS);
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kPackedWaves * G), LDS, s, p);
-  return launch_status("packed_fwd");
-}
-
 template <bool F16, int D>
-static int dispatch_packed_fwd(PackedParams p, hipStream_t s) {
+static int launch_packed_fwd(const PackedParams& p, hipStream_t s) {
+  constexpr int LDS = packed_fwd_lds<D>();
+  static_assert(LDS <= 65536, "LDS within the default limit");
   const int64_t grid = packed_grid(p.tq, p.n, p.heads, p.split_least > 0);
-  // Two key groups halve the longest workgroup's time, which is the launch's where the chip holds all of them at once (one
-  // prompt of 4096 tokens, 12 heads of 128: 80.2 -> 65.7 us, of 2048: 38.8 -> 34.7); with more workgroups, the barriers that
-  // eight waves share cost (8192 tokens 214.6 -> 224.4 us), for short prompts the join does (four of up to 200 tokens, 64
-  // wide: 8.9 -> 9.6 us), and parts of tiles do more for the longest (2 heads, 16384 tokens: 204 us so, 180 in parts).
-  const bool two = p.split_least == 0 && grid <= 512 && p.tk >= 768ll * p.n;
-  const int rc = two ? launch_packed_fwd<F16, D, 2>(p, grid, s) : launch_packed_fwd<F16, D, 1>(p, grid, s);
+  hipLaunchKernelGGL((packed_fwd_kernel<F16, D>), dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS, s, p);
+  const int rc = launch_status("packed_fwd");
   if (rc != VMO_OK || p.split_least == 0) return rc;
-  const int64_t slots = (kPackedParts + p.heads - 1) / p.heads * p.heads;
-  hipLaunchKernelGGL((packed_fwd_join_kernel<F16, D>), dim3((unsigned)slots), dim3(256), kPackedSeqBytes * kPackedMaxSeqs, s, p);
+  hipLaunchKernelGGL((packed_fwd_join_kernel<F16, D>), dim3(kPackedParts), dim3(256), 0, s, p);
   return launch_status("packed_fwd_join");
 }
 
 int packed_fwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s) {
-  if (d == 64) return f16 ? dispatch_packed_fwd<true, 64>(p, s) : dispatch_packed_fwd<false, 64>(p, s);
-  return f16 ? dispatch_packed_fwd<true, 128>(p, s) : dispatch_packed_fwd<false, 128>(p, s);
+  if (d == 64) return f16 ? launch_packed_fwd<true, 64>(p, s) : launch_packed_fwd<false, 64>(p, s);
+  return f16 ? launch_packed_fwd<true, 128>(p, s) : launch_packed_fwd<false, 128>(p, s);
 }
 
 }  // namespace vmo
