@@ -26,7 +26,7 @@ struct PackedParams {
   int64_t st_sh;
   float* neg_delta;                        // (heads, tq): -rowsum(o dO), from the dq kernel to the dk / dv one
   float *part, *part2;                     // parts of split tiles: (slots, 128, D) fp32 sums; the forward's m and l (.., 2), or dv's
-                                           // (splits > 1: dk's and dv's (splits, kv_heads, tk, D))
+  float *sum, *sum2;                       // splits > 1: dk's and dv's (splits, kv_heads, tk, D) fp32
   i32x4* records;                          // of the first kPackedParts workgroups: first row, rows, part and parts of its tile
   int splits;                              // dk / dv: workgroups that share a key tile, each with group / splits of the heads
   int split_least;                         // tiles of up to so many units are never split (0: no tile is)

@@ -54,15 +54,14 @@ constexpr int64_t kRecordFloats = (int64_t)kPackedParts * 4;
 static int64_t fwd_layout(const vmo_packed_args* a) {
   return packed_splits(a->tk) ? (kRecordFloats + part_floats(a->d) + part_floats(2)) * 4 : 0;
 }
-struct BwdLayout { int64_t delta, kv, bytes; int splits; };   // floats of -delta and of dk's parts
+struct BwdLayout { int64_t delta, part, sum, bytes; int splits; };   // floats of -delta, of dk's parts and of its shares' sums
 static BwdLayout bwd_layout(const vmo_packed_args* a) {
   BwdLayout l;
   l.delta = ((int64_t)a->heads * a->tq + 63) / 64 * 64;
   l.splits = packed_bwd_splits(a->tk, a->kv_heads, a->heads / a->kv_heads);
-  const int64_t q = packed_splits(a->tk) ? part_floats(a->d) : 0;
-  l.kv = l.splits > 1 ? (int64_t)l.splits * a->kv_heads * a->tk * a->d
-         : packed_splits(a->tq) ? part_floats(a->d) : 0;
-  l.bytes = (kRecordFloats + l.delta + (q > 2 * l.kv ? q : 2 * l.kv)) * 4;
+  l.part = packed_splits(a->tk) || packed_splits(a->tq) ? part_floats(a->d) : 0;
+  l.sum = l.splits > 1 ? (int64_t)l.splits * a->kv_heads * a->tk * a->d : 0;
+  l.bytes = (kRecordFloats + l.delta + 2 * l.part + 2 * l.sum) * 4;
   return l;
 }
 static bool sizes_ok(const vmo_packed_args* a) {
@@ -113,6 +112,8 @@ extern "C" int vmo_packed_bwd(const vmo_packed_args* a, void* stream) {
   p.records = (i32x4*)a->workspace;
   p.neg_delta = (float*)a->workspace + kRecordFloats;
   p.part = p.neg_delta + l.delta;
-  p.part2 = p.part + l.kv;
+  p.part2 = p.part + l.part;
+  p.sum = p.part2 + l.part;
+  p.sum2 = p.sum + l.sum;
   return packed_bwd_launch(p, a->dtype == VMO_DTYPE_F16, a->d, (hipStream_t)stream);
 }

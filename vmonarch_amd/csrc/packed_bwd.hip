@@ -385,9 +385,10 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   VMO_LDS float* patch = (VMO_LDS float*)(smem + wave * kEpiPatchBytes);
   const int nrows = min(32, nk - k0);
   if (parts > 1 || p.splits > 1) {
-    const int64_t r = (p.splits > 1 ? (int64_t)(split * p.kv_heads + kvh) * p.tk + kb + k0 : (int64_t)blockIdx.x * kPackedTile + wave * 32) * D;
-    store_acc_rows<F16>(patch, dk, NA, p.sm_scale, kGradStoreF32, (char*)(p.part + r), D * 4, nrows, lane);
-    store_acc_rows<F16>(patch, dv, NA, 1.0f, kGradStoreF32, (char*)(p.part2 + r), D * 4, nrows, lane);
+    const bool slot = parts > 1;
+    const int64_t r = (slot ? (int64_t)blockIdx.x * kPackedTile + wave * 32 : (int64_t)(split * p.kv_heads + kvh) * p.tk + kb + k0) * D;
+    store_acc_rows<F16>(patch, dk, NA, p.sm_scale, kGradStoreF32, (char*)((slot ? p.part : p.sum) + r), D * 4, nrows, lane);
+    store_acc_rows<F16>(patch, dv, NA, 1.0f, kGradStoreF32, (char*)((slot ? p.part2 : p.sum2) + r), D * 4, nrows, lane);
   } else {
     store_acc_rows<F16>(patch, dk, NA, p.sm_scale, kGradStore,
                         (char*)((T*)p.dk + (int64_t)kvh * p.dk_sh + (int64_t)(kb + k0) * p.dk_sn), p.dk_sn * 2, nrows, lane);
@@ -405,16 +406,23 @@ __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams p) {
   constexpr int TPR = D / 4;
   const i32x4 rec = p.records[blockIdx.x];   // first row, rows, part, parts
   if (rec[3] <= 1) return;
-  const int heads = KEYS ? p.kv_heads : p.heads, head = packed_head((int)blockIdx.x % heads, heads), parts = rec[3];
-  const int d4 = (threadIdx.x % TPR) * 4;
-  const int64_t slot0 = (int)blockIdx.x - rec[2] * heads;
+  const int shares = KEYS ? p.kv_heads * p.splits : p.heads, hs = packed_head((int)blockIdx.x % shares, shares), parts = rec[3];
+  const int head = KEYS ? hs / p.splits : hs, d4 = (threadIdx.x % TPR) * 4;
+  const int64_t slot0 = (int)blockIdx.x - rec[2] * shares;
   for (int r = rec[2] * rec[1] / parts + threadIdx.x / TPR; r < (rec[2] + 1) * rec[1] / parts; r += 256 / TPR) {
     f32x4 a = f32x4{}, b = f32x4{};
 #pragma unroll 4
     for (int i = 0; i < parts; ++i) {
-      const int64_t at = ((slot0 + i * heads) * kPackedTile + r) * D + d4;
+      const int64_t at = ((slot0 + i * shares) * kPackedTile + r) * D + d4;
       a += *(const f32x4*)(p.part + at);
       if constexpr (KEYS) b += *(const f32x4*)(p.part2 + at);
+    }
+    const int64_t tok = rec[0] + r;
+    if (KEYS && p.splits > 1) {   // a share's sums: packed_bwd_sum adds the shares
+      const int64_t at = ((int64_t)(hs % p.splits * p.kv_heads + head) * p.tk + tok) * D + d4;
+      *(f32x4*)(p.sum + at) = a;
+      *(f32x4*)(p.sum2 + at) = b;
+      continue;
     }
     V4 x, y;
 #pragma unroll
@@ -422,7 +430,6 @@ __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams p) {
       x[e] = to_elem<T>(a[e]);
       y[e] = to_elem<T>(b[e]);
     }
-    const int64_t tok = rec[0] + r;
     if constexpr (KEYS) {
       *(V4*)((T*)p.dk + (int64_t)head * p.dk_sh + tok * p.dk_sn + d4) = x;
       *(V4*)((T*)p.dv + (int64_t)head * p.dv_sh + tok * p.dv_sn + d4) = y;
@@ -449,8 +456,8 @@ __global__ __launch_bounds__(256) void packed_bwd_sum_kernel(PackedParams p) {
 #pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
       const int64_t at = (s * rows + r) * D + c4;
-      a += *(const f32x4*)(p.part + at);
-      b += *(const f32x4*)(p.part2 + at);
+      a += *(const f32x4*)(p.sum + at);
+      b += *(const f32x4*)(p.sum2 + at);
     }
   V4 x, y;
 #pragma unroll
@@ -462,9 +469,9 @@ __global__ __launch_bounds__(256) void packed_bwd_sum_kernel(PackedParams p) {
   *(V4*)((T*)p.dv + (int64_t)kvh * p.dv_sh + (int64_t)tok * p.dv_sn + c4) = y;
 }
 
-// Workgroups that share a key tile: as many as divide the group and bring the launch to two rounds of the chip's slots.  With
-// shared heads this balances better than parts of a tile do, whose queries every XCD's L2 would have to hold (8 heads over 2,
-// prompts of 12000 and 4384 tokens: 651 us so, 790 in parts).
+// Workgroups that share a key tile, each with some of the group's heads: as many as divide the group and bring the launch to
+// two rounds of the chip's slots.  Where heads are shared this comes before parts of a tile, whose queries every XCD's L2 would
+// have to hold (8 heads over 2, prompts of 12000 and 4384 tokens: 651 us so, 790 in parts alone).
 int packed_bwd_splits(int64_t tk, int kv_heads, int group) {
   const int64_t tiles = ((tk + kPackedTile - 1) / kPackedTile) * kv_heads;
   int splits = 1;
@@ -498,13 +505,13 @@ static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   if (LDS_KV > 65536 &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_KV) != hipSuccess)
     return set_error(VMO_ERR_LAUNCH, "packed_bwd: cannot raise the LDS limit to %d bytes", LDS_KV);
-  p.split_least = p.splits == 1 && packed_splits(p.tq) ? kPackedSplit : 0;
+  p.split_least = packed_splits(p.tq) ? kPackedSplit : 0;
   const int64_t grid = packed_grid(p.tk, p.n, p.kv_heads * p.splits, p.split_least > 0);
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_KV, s, p);
   rc = launch_status("packed_bwd_dkdv");
   if (rc != VMO_OK) return rc;
-  if (p.split_least > 0) return join(packed_bwd_join_kernel<F16, D, true>);
-  if (p.splits == 1) return VMO_OK;
+  if (p.split_least > 0) rc = join(packed_bwd_join_kernel<F16, D, true>);
+  if (rc != VMO_OK || p.splits == 1) return rc;
   const int64_t threads = (int64_t)p.kv_heads * p.tk * (D / 4);
   hipLaunchKernelGGL((packed_bwd_sum_kernel<F16, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
   return launch_status("packed_bwd_sum");
