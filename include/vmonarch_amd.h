@@ -330,6 +330,8 @@ int vmo_lstep_bwd_delta(const vmo_lstep_bwd_args* args, void* stream);
  * Views: stride_b is not used; q, o, grad_o, grad_q (heads, tq, d), the others (kv_heads, tk, d).  d is 64 or 128.  The
  * offsets (n + 1 int32 each, not falling) are read on the GPU and cut to [0, tq] and [0, tk]; n is at most 2048.  lse:
  * (heads, tq) fp32, log2 units, rows stat_stride apart (the forward's output, may be null there; the backward's input).
+ * o_low (may be null): o's rounding error in the same type and layout as o, written by the forward and read by the backward,
+ * whose delta is then that of the unrounded o.
  * zero_rest: rows of o outside every sequence are written as zeros (else they are left as they were); the backward always
  * writes zeros to such rows of its gradients.
  */
@@ -337,6 +339,7 @@ enum { VMO_PACKED_MAX_SEQUENCES = 2048 };
 typedef struct vmo_packed_args {
   int32_t dtype, heads, kv_heads, n, tq, tk, d, causal, zero_rest;
   vmo_view q, k, v, o;
+  void* o_low;
   const int32_t *q_offsets, *k_offsets;
   float* lse;
   int64_t stat_stride;

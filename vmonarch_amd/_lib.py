@@ -81,7 +81,7 @@ class LstepBwdArgs(ctypes.Structure):
 class PackedArgs(ctypes.Structure):
     _fields_ = [
         ("dtype", c_int32), ("heads", c_int32), ("kv_heads", c_int32), ("n", c_int32), ("tq", c_int32), ("tk", c_int32),
-        ("d", c_int32), ("causal", c_int32), ("zero_rest", c_int32), ("q", View), ("k", View), ("v", View), ("o", View),
+        ("d", c_int32), ("causal", c_int32), ("zero_rest", c_int32), ("q", View), ("k", View), ("v", View), ("o", View), ("o_low", c_void_p),
         ("q_offsets", c_void_p), ("k_offsets", c_void_p), ("lse", c_void_p), ("stat_stride", c_int64), ("sm_scale", c_float),
         ("grad_o", View), ("grad_q", View), ("grad_k", View), ("grad_v", View), ("workspace", c_void_p),
         ("workspace_bytes", c_size_t),

@@ -637,8 +637,8 @@ void packed_checks(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   require(q_off.size(0) >= 1 && q_off.size(0) == k_off.size(0), "offsets: one more than the sequences, as many for keys as for queries");
 }
 
-std::tuple<Tensor, OptT> packed_fwd(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& q_off,
-                                    const Tensor& k_off, double sm_scale, bool causal, const OptT& out, bool want_lse) {
+std::tuple<Tensor, OptT, OptT> packed_fwd(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& q_off,
+                                    const Tensor& k_off, double sm_scale, bool causal, const OptT& out, bool train) {
   packed_checks(q_in, k_in, v_in, q_off, k_off);
   if (out) {
     like(q_in, *out);
@@ -649,8 +649,10 @@ std::tuple<Tensor, OptT> packed_fwd(const Tensor& q_in, const Tensor& k_in, cons
   const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
   vmo_packed_args a = packed_args(q, k, v, q_off, k_off, sm_scale, causal);
   const Tensor o = out ? *out : empty_rows(q);
-  OptT lse;
-  if (want_lse) {
+  OptT lse, low;   // what the backward needs beside o
+  if (train) {
+    low = empty_rows(o);
+    a.o_low = low->data_ptr();
     lse = at::empty({q.size(0), q.size(1)}, f32(q));
     a.lse = lse->data_ptr<float>();
     a.stat_stride = q.size(1);
@@ -664,23 +666,24 @@ std::tuple<Tensor, OptT> packed_fwd(const Tensor& q_in, const Tensor& k_in, cons
     a.workspace_bytes = bytes;
   }
   check(vmo_packed_fwd(&a, stream_of(q)), "vmo_packed_fwd");
-  return {o, lse};
+  return {o, low, lse};
 }
 
-std::tuple<Tensor, Tensor, Tensor> packed_bwd(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o_in,
-                                              const Tensor& lse, const Tensor& dO_in, const Tensor& q_off, const Tensor& k_off,
+std::tuple<Tensor, Tensor, Tensor> packed_bwd(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& o,
+                                              const Tensor& low, const Tensor& lse, const Tensor& dO_in, const Tensor& q_off, const Tensor& k_off,
                                               double sm_scale, bool causal) {
   packed_checks(q_in, k_in, v_in, q_off, k_off);
-  like(q_in, {&o_in, &dO_in});
+  like(q_in, {&o, &low, &dO_in});
   same_device(q_in, lse);
-  require(o_in.sizes() == q_in.sizes() && dO_in.sizes() == q_in.sizes(), "o and its gradient are shaped like q");
+  require(o.sizes() == q_in.sizes() && dO_in.sizes() == q_in.sizes(), "o and its gradient are shaped like q");
+  require(low.sizes() == o.sizes() && low.strides() == o.strides(), "low is the forward's");
   require(lse.dim() == 2 && lse.size(0) == q_in.size(0) && lse.size(1) == q_in.size(1) && lse.is_contiguous() &&
               lse.scalar_type() == at::kFloat, "lse is the forward's");
   const OnGpuOf device(q_in);
-  const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in), o = readable(o_in), dO = readable(dO_in);
+  const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in), dO = readable(dO_in);
   vmo_packed_args a = packed_args(q, k, v, q_off, k_off, sm_scale, causal);
   const Tensor dq = empty_rows(q_in), dk = empty_rows(k_in), dv = empty_rows(v_in);
-  a.o = rows_view(o); a.grad_o = rows_view(dO);
+  a.o = rows_view(o); a.o_low = low.data_ptr(); a.grad_o = rows_view(dO);
   a.grad_q = rows_view(dq); a.grad_k = rows_view(dk); a.grad_v = rows_view(dv);
   a.lse = lse.data_ptr<float>();
   a.stat_stride = lse.size(1);

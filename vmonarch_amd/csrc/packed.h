@@ -17,6 +17,7 @@ constexpr int kPackedWaves = 4;
 struct PackedParams {
   const void *q, *k, *v, *o, *dO;
   void *out, *dq, *dk, *dv;
+  void* o_low;                             // o's rounding error in 16 bits, laid out as o (or null): delta is of the unrounded o
   int64_t q_sh, q_sn, k_sh, k_sn, v_sh, v_sn, o_sh, o_sn, do_sh, do_sn;
   int64_t dq_sh, dq_sn, dk_sh, dk_sn, dv_sh, dv_sn;
   const int32_t *q_off, *k_off;
@@ -128,21 +129,24 @@ constexpr int kPackedSeqBytes = 16;   // LDS of a sequence while a workgroup fin
 // The idx-th part over all sequences' tiles, heaviest tiles first (a tile's time is its keys, or queries: with the heavy ones
 // first the chip's last round is made of light ones); `heads` workgroups take each.  The largest level whose parts and those
 // above are more than idx is found by bisection over per-sequence counts, from rows and keys that lie in LDS (free again
-// after the call); a level holds the sequences in order.  Every wave does the same.
+// after the call) where there are more than 64; a level holds the sequences in order.  Every wave does the same.
 template <bool KEYS>
 __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int idx, int blocks, int heads, VMO_LDS int* lds) {
   const int lane = threadIdx.x & 63;
-  for (int s = threadIdx.x; s < p.n; s += (int)blockDim.x) {
-    const PackedSeq q = packed_seq(p, s);
-    *(VMO_LDS i32x4*)(lds + 4 * s) = i32x4{q.qb, q.nq, q.kb, q.nk};
+  const bool few = p.n <= 64;   // one a lane: each wave reads them itself
+  if (!few) {
+    for (int s = threadIdx.x; s < p.n; s += (int)blockDim.x) {
+      const PackedSeq q = packed_seq(p, s);
+      *(VMO_LDS i32x4*)(lds + 4 * s) = i32x4{q.qb, q.nq, q.kb, q.nk};
+    }
+    __syncthreads();
   }
-  __syncthreads();
   auto seq = [&](int s) __attribute__((always_inline)) {
     const i32x4 x = *(const VMO_LDS i32x4*)(lds + 4 * s);
     return PackedSeq{x[0], x[1], x[2], x[3]};
   };
-  // (up to 64 sequences: one a lane, in registers)
-  const PackedSeq mine = lane < p.n ? seq(lane) : PackedSeq{0, 0, 0, 0};
+  PackedSeq mine{0, 0, 0, 0};
+  if (lane < p.n) mine = few ? packed_seq(p, lane) : seq(lane);
   const PackedTiles first = packed_tiles<KEYS>(p, mine);
   int best = first.tiles > 0 ? min(first.top, first.cap) : 0;
   float work = packed_work(first);
@@ -210,7 +214,7 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
       left -= sum;
     }
   }
-  __syncthreads();   // every wave has read the sequences
+  if (!few) __syncthreads();   // every wave has read the sequences
   return r;
 }
 

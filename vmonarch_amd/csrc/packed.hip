@@ -25,6 +25,7 @@ static int packed_prepare(const vmo_packed_args* a, bool bwd, const char* what, 
         return set_error(VMO_ERR_INVALID, "%s: tensors need 16-byte aligned rows (strides multiple of 8 elements)", what);
       if (x->stride_n >= kMaxRowStride) return set_error(VMO_ERR_UNSUPPORTED, "%s: row stride must be below 2^27 elements", what);
     }
+  if (a->o_low && !aligned16(a->o_low)) return set_error(VMO_ERR_INVALID, "%s: o_low needs 16-byte alignment", what);
   if (bwd && a->tq > 0 && !a->lse) return set_error(VMO_ERR_INVALID, "%s: needs the forward's lse", what);
   const int64_t tiles = ((int64_t)(a->tq > a->tk ? a->tq : a->tk) + kPackedTile - 1) / kPackedTile + a->n;
   if (a->tq > (1 << 26) || a->tk > (1 << 26) || tiles * a->heads > (1ll << 30))   // (counts of tiles stay within 32 bits)
@@ -38,6 +39,7 @@ static int packed_prepare(const vmo_packed_args* a, bool bwd, const char* what, 
   p.dq_sh = a->grad_q.stride_h; p.dq_sn = a->grad_q.stride_n;
   p.dk_sh = a->grad_k.stride_h; p.dk_sn = a->grad_k.stride_n;
   p.dv_sh = a->grad_v.stride_h; p.dv_sn = a->grad_v.stride_n;
+  p.o_low = a->o_low;
   p.q_off = a->q_offsets; p.k_off = a->k_offsets;
   p.n = a->n; p.tq = a->tq; p.tk = a->tk; p.heads = a->heads; p.kv_heads = a->kv_heads; p.group = a->heads / a->kv_heads;
   p.causal = a->causal != 0; p.zero_rest = a->zero_rest != 0;

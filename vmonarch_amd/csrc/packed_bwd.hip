@@ -10,7 +10,9 @@
 // Where some workgroups have far more to do than others, heavy tiles are split (packed.h; dk / dv: over the group's heads
 // first), into fp32 sums that packed_bwd_join (or packed_bwd_sum) adds in order.
 // Stages that a wave does not see at all are skipped, those on the diagonal (or at a sequence's end) masked.
-// P and dS are rounded to the 16-bit type as operands, the gradients once at the end.
+// P and dS are rounded to the 16-bit type as operands, the gradients once at the end.  delta takes o as it was before its
+// rounding, from the forward's o and the rounding's error beside it: with the rounded o alone, delta's error was a third of
+// what the roundings of dS and of the gradients give (fp16, dq and dk: 1.52 times the error of one rounding, @@ so).
 #include "packed.h"
 
 namespace vmo {
@@ -77,6 +79,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
     const T* qp = (const T*)p.q + (int64_t)head * p.q_sh + tok * p.q_sn + hl * 8;
     const T* dp = (const T*)p.dO + (int64_t)head * p.do_sh + tok * p.do_sn + hl * 8;
     const T* op = (const T*)p.o + (int64_t)head * p.o_sh + tok * p.o_sn + hl * 8;
+    const T* lp = p.o_low ? (const T*)p.o_low + (int64_t)head * p.o_sh + tok * p.o_sn + hl * 8 : nullptr;
 #pragma unroll
     for (int ds = 0; ds < NDS; ++ds) {
       qf[ds] = *(const V8*)(qp + ds * 16);
@@ -86,9 +89,9 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
     for (int ds = 0; ds < NDS; ++ds) {
       dof[ds] = *(const V8*)(dp + ds * 16);
       asm volatile("" : "+v"(dof[ds]));
-      const V8 y = *(const V8*)(op + ds * 16);
+      const V8 y = *(const V8*)(op + ds * 16), z = lp ? *(const V8*)(lp + ds * 16) : V8{};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) delta = fmaf((float)dof[ds][e], (float)y[e], delta);
+      for (int e = 0; e < 8; ++e) delta = fmaf((float)dof[ds][e], (float)y[e] + (float)z[e], delta);
     }
   }
   float alpha = -wave_sum32(delta);

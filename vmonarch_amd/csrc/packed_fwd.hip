@@ -296,6 +296,17 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
   const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;   // (a row that sees no key)
   T* out = (T*)p.out + (int64_t)head * p.o_sh + (int64_t)(qb + q0) * p.o_sn;
   store_acc_rows<F16>(patch, acc, NA, inv, kGradStore, (char*)out, p.o_sn * 2, nrows, lane);
+  if (p.o_low) {
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = acc[a][r] * inv;
+        acc[a][r] = x - (float)to_elem<T>(x);
+      }
+    T* low = (T*)p.o_low + (int64_t)head * p.o_sh + (int64_t)(qb + q0) * p.o_sn;
+    store_acc_rows<F16>(patch, acc, NA, 1.f, kGradStore, (char*)low, p.o_sn * 2, nrows, lane);
+  }
   if (p.lse && hl == 0 && l32 < nrows)
     p.lse[(int64_t)head * p.st_sh + qb + q0 + l32] = l_tot == 0.f ? 0.f : m_run + fast_log2(l_tot);
 }
@@ -324,11 +335,16 @@ __global__ __launch_bounds__(256) void packed_fwd_join_kernel(PackedParams p) {
       for (int e = 0; e < 4; ++e) acc[e] = fmaf(acc[e], f, y[e] * pf);
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    typename Elem<F16>::V4 y;
+    typename Elem<F16>::V4 y, low;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = to_elem<T>(acc[e] * inv);
-    const int64_t tok = rec[0] + r;
-    *(typename Elem<F16>::V4*)((T*)p.out + (int64_t)head * p.o_sh + tok * p.o_sn + d4) = y;
+    for (int e = 0; e < 4; ++e) {
+      const float x = acc[e] * inv;
+      y[e] = to_elem<T>(x);
+      low[e] = to_elem<T>(x - (float)y[e]);
+    }
+    const int64_t tok = rec[0] + r, at = (int64_t)head * p.o_sh + tok * p.o_sn + d4;
+    *(typename Elem<F16>::V4*)((T*)p.out + at) = y;
+    if (p.o_low) *(typename Elem<F16>::V4*)((T*)p.o_low + at) = low;
     if (p.lse && d4 == 0) p.lse[(int64_t)head * p.st_sh + tok] = l == 0.f ? 0.f : m + fast_log2(l);
   }
 }

@@ -10,16 +10,16 @@ from .kernel import _recorded
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, k_offsets, sm_scale, causal):
-        o, lse = _lib.host().packed_fwd(q, k, v, offsets, k_offsets, sm_scale, causal, None, True)
-        ctx.save_for_backward(q, k, v, o, lse, offsets, k_offsets)
+        o, low, lse = _lib.host().packed_fwd(q, k, v, offsets, k_offsets, sm_scale, causal, None, True)
+        ctx.save_for_backward(q, k, v, o, low, lse, offsets, k_offsets)
         ctx.sm_scale, ctx.causal = sm_scale, causal
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, offsets, k_offsets = ctx.saved_tensors
-        return (*_lib.host().packed_bwd(q, k, v, o, lse, do.to(q.dtype), offsets, k_offsets, ctx.sm_scale, ctx.causal),
+        q, k, v, o, low, lse, offsets, k_offsets = ctx.saved_tensors
+        return (*_lib.host().packed_bwd(q, k, v, o, low, lse, do.to(q.dtype), offsets, k_offsets, ctx.sm_scale, ctx.causal),
                 None, None, None, None)
 
 
