@@ -194,7 +194,7 @@ def test_replays_with_other_lengths_from_a_graph():
 
     def step():
         o = packed_attention(*leaves, off)
-        return [o, *torch.autograd.grad(o, leaves, grad)]
+        return [o.detach(), *torch.autograd.grad(o, leaves, grad)]
 
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
@@ -238,3 +238,51 @@ def test_gradient_against_differences():
         diff = (value(1e-4) - value(-1e-4)) / 2e-4
         ours, allowed = float((got[i].double() * d).sum()), float((want[name][1] * d.abs()).sum())
         assert abs(ours - diff) <= allowed + 1e-5 * abs(diff)
+
+
+def test_capture_beside_a_live_eager_graph_is_refused():
+    """The leaf's gradient node belongs to the eager graph's stream: a captured backward would end the process."""
+    from vmonarch_amd import packed_attention
+    g = torch.Generator().manual_seed(7)
+    leaves = [tensor(g, h, 50, 64, torch.bfloat16, "hnd").requires_grad_() for h in (2, 1, 1)]
+    grad, off = tensor(g, 2, 50, 64, torch.bfloat16, "hnd"), offsets([50])
+    alive = packed_attention(*leaves, off)
+    torch.cuda.synchronize()
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(4, device=DEV)
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="another stream"):
+            packed_attention(*leaves, off)
+        with torch.no_grad():
+            o = packed_attention(*leaves, off)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, alive) and float(x[0]) == 1
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = packed_attention(*leaves, off)
+        got = torch.autograd.grad(o, leaves, grad)
+    del o
+    graph.replay()
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(packed_attention(*leaves, off), leaves, grad)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_on_another_stream():
+    """Work and allocations on the stream that is current; the result of a call on one stream used on another after a wait."""
+    from vmonarch_amd import packed_attention
+    g = torch.Generator().manual_seed(11)
+    q, k, v = (tensor(g, h, 3000, 64, torch.bfloat16, "nhd") for h in (2, 1, 1))
+    off = offsets([2000, 1000])
+    want = packed_attention(q, k, v, off)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams * 2:                       # two calls at once, their workspaces apart
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(packed_attention(q, k, v, off))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)

@@ -16,7 +16,10 @@
 #include <Python.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -617,6 +620,21 @@ void index_list(const Tensor& q, const Tensor& t, int64_t dims, const char* msg)
   same_device(q, t);
 }
 
+// A leaf has one node that its gradients go to, made on the stream of the first graph that records it and kept while any
+// lives.  A captured backward would have the stream of an eager one wait on it, which capture forbids, and the autograd
+// engine's thread then ends the process: refused here, before anything is recorded.
+void leaves_fit_capture(std::initializer_list<const Tensor*> ts) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor* t : ts) {
+    if (!t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    if (stream && stream->id() != c10::hip::getCurrentHIPStream(t->device().index()).id())   // (torch calls the device type CUDA)
+      throw std::runtime_error("vmonarch_amd: an autograd graph of another stream holds q, k or v: delete its results before "
+                               "capturing their gradients");
+  }
+}
+
 vmo_packed_args packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_off, const Tensor& k_off,
                             double sm_scale, bool causal) {
   vmo_packed_args a{};
@@ -651,6 +669,7 @@ std::tuple<Tensor, OptT, OptT> packed_fwd(const Tensor& q_in, const Tensor& k_in
   const Tensor o = out ? *out : empty_rows(q);
   OptT lse, low;   // what the backward needs beside o
   if (train) {
+    leaves_fit_capture({&q_in, &k_in, &v_in});
     low = empty_rows(o);
     a.o_low = low->data_ptr();
     lse = at::empty({q.size(0), q.size(1)}, f32(q));

@@ -44,7 +44,8 @@ def packed_attention(q, k, v, offsets, k_offsets=None, sm_scale=None, causal=Tru
     The offsets are read on the GPU when the kernels run: a captured graph replays with what they then hold, and what
     reaches outside the tensors is cut.  They must not fall from one sequence to the next; at most 2048 sequences a call.
     What a row does not see -- later tokens, other sequences, rows behind the last one -- has no part in its result,
-    infinities and NaN included.  To capture the backward in a graph, take the gradients with torch.autograd.grad.
+    infinities and NaN included.  To capture the backward in a graph, take the gradients with torch.autograd.grad, of leaves
+    that no eager graph of another stream still holds (where q, k or v is such a leaf the capture is refused).
     """
     if k_offsets is None:
         k_offsets = offsets
