@@ -286,3 +286,49 @@ def test_on_another_stream():
             outs.append(packed_attention(q, k, v, off))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def test_no_keys_and_no_sequences():
+    from vmonarch_amd import packed_attention
+    q = torch.ones(2, 30, 64, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    k = torch.ones(1, 0, 64, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    none = torch.zeros(2, device=DEV, dtype=torch.int32)
+    for off, koff in ((offsets([30]), none), (none[:1], none[:1])):
+        o = packed_attention(q, k, k, off, koff)
+        assert not bool(o.any())
+        dq, dk = torch.autograd.grad(o.sum(), (q, k))
+        assert not bool(dq.any()) and dk.shape == k.shape
+    kk = torch.ones(1, 40, 64, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    e = torch.ones(2, 0, 64, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    o = packed_attention(e, kk, kk, none, offsets([40]))
+    assert o.shape == e.shape and not bool(torch.autograd.grad(o.sum(), kk)[0].any())
+    assert not bool(torch.autograd.grad(packed_attention(q, kk, kk, none[:1], none[:1]).sum(), kk)[0].any())
+
+
+def test_inputs_that_the_kernels_cannot_read_in_place():
+    """Features apart, rows off 16 bytes, heads or rows expanded: copied, with the results of contiguous tensors."""
+    from vmonarch_amd import packed_attention
+    g = torch.Generator().manual_seed(21)
+    base = torch.randn(4, 90, 128, generator=g).bfloat16().to(DEV)
+    off = offsets([90])
+    apart = base[:, :, ::2]
+    odd = torch.empty(4 * 90 * 64 + 3, device=DEV, dtype=torch.bfloat16)[3:].view(4, 90, 64).copy_(apart)
+    heads, rows = base[:1, :, :64].expand(4, 90, 64), base[:, :1, :64].expand(4, 90, 64)
+    for q in (apart, odd, heads, rows):
+        for k in (apart, odd, heads, rows):
+            leaves = [t.detach().requires_grad_() for t in (q, k, odd)]
+            plain = [t.detach().contiguous().clone().requires_grad_() for t in (q, k, odd)]
+            o, want = (packed_attention(*x, off) for x in (leaves, plain))
+            assert torch.equal(o, want)
+            for a, b in zip(torch.autograd.grad(o.sum(), leaves), torch.autograd.grad(want.sum(), plain)):
+                assert torch.equal(a, b)
+
+
+def test_a_buffer_that_is_written_counts_as_changed():
+    from vmonarch_amd import packed_attention
+    q = torch.ones(1, 10, 64, device=DEV, dtype=torch.bfloat16)
+    out = torch.ones_like(q)
+    y = (out * torch.ones_like(q).requires_grad_()).sum()
+    packed_attention(q, q, q, offsets([10]), out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

@@ -16,7 +16,8 @@ def i32(*values):
     (dict(k=x(3, 9, 64), v=x(3, 9, 64)), "multiple"), (dict(v=x(2, 8, 64)), "one shape"), (dict(k=x(2, 9, 32), v=x(2, 9, 32)), "head dim"),
     (dict(q=x(1, 4, 9, 64)), "heads, tokens, D"), (dict(offsets=torch.tensor([0, 9])), "int32"), (dict(offsets=i32()), "one more"),
     (dict(k_offsets=i32(0, 4, 9)), "one more"), (dict(out=x(4, 8, 64)), "shaped like q"), (dict(out=x(4, 9, 64, dtype=torch.float16)), "dtype"),
-    (dict(k=torch.zeros(2, 9, 64, dtype=torch.bfloat16, device="meta")), "device")])
+    (dict(k=torch.zeros(2, 9, 64, dtype=torch.bfloat16, device="meta")), "device"),
+    ({n: x(h, 9, 64, dtype=torch.float32) for n, h in (("q", 4), ("k", 2), ("v", 2))}, "bf16 or fp16")])
 def test_packed_attention_refuses(change, message):
     from vmonarch_amd import packed_attention
     args = dict(q=x(4, 9, 64), k=x(2, 9, 64), v=x(2, 9, 64), offsets=i32(0, 9))
@@ -183,4 +184,55 @@ def test_the_cache_refuses():
         books(page=12)
     with pytest.raises(ValueError):
         books(pages=0)
+    from vmonarch_amd import PagedKVCache
+    with pytest.raises(ValueError, match="bf16 and fp16"):
+        PagedKVCache(4, 8, 1, 64, dtype=torch.float32, device="cpu")
     assert c.compact() == 0
+
+
+def test_forks_copy_a_page_that_others_hold_when_they_write(monkeypatch):
+    """Which pages are copied, and who keeps the first one: three sequences over one unfilled page."""
+    import vmonarch_amd.paged as paged
+    copies = []
+    monkeypatch.setattr(paged, "copy_pages", lambda k, v, src, dst: copies.append((list(src), list(dst))))
+    c = books(pages=10)
+    a = c.open()
+    c.grow([a], [11])                                  # pages 0, 1; 1 holds 3 tokens
+    b, d = c.fork(a), c.fork(a)
+    c.grow([b])                                        # one writes: a copy of its own
+    assert copies == [([1], [2])] and c.pages_of(b) == [0, 2] and c.pages_of(a) == c.pages_of(d) == [0, 1]
+    c.grow([a, d])                                     # both that are left: one copies, one keeps
+    assert copies[1:] == [([1], [3])] and c.pages_of(a) == [0, 3] and c.pages_of(d) == [0, 1]
+    c.grow([a, b, d])
+    assert len(copies) == 2
+    e = c.fork(a)
+    c.grow([e], [0])                                   # nothing written: still shared
+    assert c.pages_of(e) == c.pages_of(a) and len(copies) == 2
+    full = c.open()
+    c.grow([full], [8])
+    other = c.fork(full)
+    c.grow([full, other])                              # a filled page stays shared
+    assert len(copies) == 2 and c.pages_of(full)[0] == c.pages_of(other)[0] and c.pages_of(full)[1] != c.pages_of(other)[1]
+    for s in (a, b, d, e, full, other):
+        c.free(s)
+    assert c.free_pages == 10
+
+
+def test_compaction_moves_the_held_pages_down(monkeypatch):
+    import vmonarch_amd.paged as paged
+    moves = []
+    monkeypatch.setattr(paged, "copy_pages", lambda k, v, src, dst: moves.append(dict(zip(src, dst))))
+    c = books(pages=12)
+    a, b, d = c.open(), c.open(), c.open()
+    for s in (a, b, d):
+        c.grow([s], [24])                              # pages 0-2, 3-5, 6-8
+    twin = c.fork(d)
+    c.free(a)
+    c.free(b)
+    assert c.compact() == 3 and moves == [{6: 0, 7: 1, 8: 2}]
+    assert c.pages_of(d) == c.pages_of(twin) == [0, 1, 2] and c.free_pages == 9
+    assert c.compact() == 0
+    c.free(d)
+    assert c.free_pages == 9
+    c.free(twin)
+    assert c.free_pages == 12 and c.grow([c.open()], [8 * 12])[0].tolist() == [list(range(12))]

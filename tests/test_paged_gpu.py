@@ -248,3 +248,76 @@ def test_token_steps_replay_from_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(o, want) and torch.equal(k.view(torch.int16), k2.view(torch.int16)), change
         _ = step(k2, v2)
+
+
+def test_a_cache_beyond_32_bits_of_bytes():
+    """Pages behind the first 4 GiB: written, copied and read where they are."""
+    from vmonarch_amd import append_pages, copy_pages, paged_attention
+    g = torch.Generator().manual_seed(31)
+    pages, KVH, page, D = 150000, 8, 16, 128            # 32 KiB a page, 4.9 GB a tensor
+    k, v = (torch.empty(pages, KVH, page, D, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    table = torch.tensor([[pages - 1, 3, pages - 7]], device=DEV, dtype=torch.int32)
+    n = 41
+    kn, vn = (torch.randn(n, KVH, D, generator=g).bfloat16().to(DEV).transpose(0, 1) for _ in range(2))
+    lens, off = torch.tensor([n], device=DEV, dtype=torch.int32), torch.tensor([0, n], device=DEV, dtype=torch.int32)
+    append_pages(kn, vn, k, v, table, lens, off)
+    assert torch.equal(k[pages - 1], kn[:, :16]) and torch.equal(v[pages - 7, :, :9], vn[:, 32:])
+    q = torch.randn(1, 16, D, generator=g).bfloat16().to(DEV)
+    o = paged_attention(q, k, v, table, lens)
+    assert_within(o[0], want_one(q[0], (kn, vn), D ** -0.5, torch.bfloat16), "high pages")
+    copy_pages(k, v, [pages - 1, pages - 7], [pages - 2, 5])
+    assert torch.equal(k[pages - 2], kn[:, :16])
+    assert torch.equal(paged_attention(q, k, v, table.new_tensor([[pages - 2, 3, 5]]), lens), o)
+
+
+def test_many_sequences():
+    """More sequences than a wave has lanes, many of them without tokens: each row whole or in parts."""
+    from vmonarch_amd import paged_attention
+    g = torch.Generator().manual_seed(33)
+    lengths = [(7 * i) % 50 if i % 3 else 0 for i in range(700)] + [3000]
+    k, v, table, lens, rows = cache(g, lengths, 1, 64, 16, torch.float16)
+    q = torch.randn(len(lengths), 4, 64, generator=g).half().to(DEV)
+    o = paged_attention(q, k, v, table, lens)
+    for b in list(range(0, 700, 13)) + [700]:
+        if lengths[b] == 0:
+            assert not bool(o[b].any())
+        else:
+            assert_within(o[b], want_one(q[b], rows[b], 64 ** -0.5, torch.float16), f"sequence {b}")
+    assert not bool(o[[i for i, n in enumerate(lengths) if n == 0]].any())
+
+
+def test_values_that_are_not_finite_stay_in_their_sequence():
+    from vmonarch_amd import paged_attention
+    g = torch.Generator().manual_seed(35)
+    k, v, table, lens, _ = cache(g, [50, 60, 70], 2, 64, 16, torch.bfloat16)
+    q = torch.randn(3, 4, 64, generator=g).bfloat16().to(DEV)
+    good = paged_attention(q, k, v, table, lens)
+    v[int(table[1, 2]), 0, 3, 7] = float("inf")
+    o = paged_attention(q, k, v, table, lens)
+    assert torch.equal(o[[0, 2]], good[[0, 2]]) and torch.equal(o[1, 2:], good[1, 2:])
+    assert bool((o[1, :2, 7] == float("inf")).all()) and torch.equal(o[1, :2, :7], good[1, :2, :7])
+    q[1] = float("nan")
+    o = paged_attention(q, k, v, table, lens)
+    assert torch.equal(o[[0, 2]], good[[0, 2]]) and torch.isnan(o[1].float()).all()
+
+
+@pytest.mark.parametrize("dtype, scale", [(torch.float16, 8.0), (torch.bfloat16, 40.0)])
+def test_sharp_rows(dtype, scale):
+    """Logits that keep growing (and falling) along the cache: the reference point moves in every wave's share."""
+    from vmonarch_amd import paged_attention
+    g = torch.Generator().manual_seed(37)
+    n, D, page = 3000, 64, 16
+    ramp = torch.linspace(-1, 1, n)[:, None] * scale / D ** 0.5
+    u = torch.finfo(dtype).eps / 2
+    for sign in (1, -1):
+        kd = (sign * ramp + 0.01 * torch.randn(n, D, generator=g)).to(dtype)
+        vd = torch.randn(n, D, generator=g).to(dtype)
+        pages = -(-n // page)
+        k, v = (torch.zeros(pages * page, D, dtype=dtype).index_copy_(0, torch.arange(n), t).view(pages, 1, page, D).to(DEV) for t in (kd, vd))
+        q = torch.ones(1, 2, D, device=DEV, dtype=dtype)
+        o = paged_attention(q, k, v, torch.arange(pages, device=DEV, dtype=torch.int32)[None], torch.tensor([n], device=DEV, dtype=torch.int32))
+        p = torch.softmax(q[0].double() @ kd.double().to(DEV).t().contiguous() * D ** -0.5, -1)
+        want, a = p @ vd.double().to(DEV), p @ vd.double().to(DEV).abs()
+        # (as for whole prompts: logits up to 2^9, fp16 weights' floor)
+        bound = u * a + u * want.abs() + 2 ** -13 * a + (n * 2.0 ** -25 * 5 if dtype == torch.float16 else 0)
+        assert bool(((o[0].double() - want).abs() <= bound).all())

@@ -597,13 +597,16 @@ bool rows_ok(const Tensor& t) {   // 16-byte aligned rows, one behind the other,
     if (t.stride(d) % 8) return false;
   return true;
 }
-Tensor readable(const Tensor& t) { return rows_ok(t) ? t : t.contiguous(); }
+Tensor readable(const Tensor& t) { return rows_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); }   // (contiguous() keeps misaligned memory)
 void writable(const Tensor& t, const char* msg) {
   if (t.numel() == 0) return;
   bool ok = rows_ok(t);
   for (int64_t d = 0; d < t.dim(); ++d) ok = ok && (t.size(d) == 1 || t.stride(d) > 0);
   if (!ok) throw py::value_error(msg);
 }
+// a tensor that a call writes in place: autograd learns of it as of torch's own in-place operations
+void written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+void sixteen_bits(const Tensor& t) { require(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, "bf16 or fp16 tensors"); }
 vmo_view rows_view(const Tensor& t) { return vmo_view{t.data_ptr(), 0, t.stride(0), t.stride(1)}; }   // (heads, tokens, D)
 vmo_view pages_view(const Tensor& t) { return vmo_view{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
 // an uninitialised tensor in the memory order of ref's (heads, tokens)
@@ -649,6 +652,7 @@ vmo_packed_args packed_args(const Tensor& q, const Tensor& k, const Tensor& v, c
 void packed_checks(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_off, const Tensor& k_off) {
   require(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "q, k and v are (heads, tokens, D)");
   like(q, {&k, &v});
+  sixteen_bits(q);
   require(k.sizes() == v.sizes() && q.size(2) == k.size(2), "k and v of one shape, q with their head dim");
   require(k.size(0) > 0 && q.size(0) > 0 && q.size(0) % k.size(0) == 0, "query heads are a multiple of the key / value heads");
   for (const Tensor* t : {&q_off, &k_off}) index_list(q, *t, 1, "offsets are int32, one-dimensional, on q's GPU");
@@ -664,6 +668,7 @@ std::tuple<Tensor, OptT, OptT> packed_fwd(const Tensor& q_in, const Tensor& k_in
     writable(*out, "vmonarch_amd: out needs 16-byte aligned rows with contiguous features");
   }
   const OnGpuOf device(q_in);
+  if (out) written(*out);
   const Tensor q = readable(q_in), k = readable(k_in), v = readable(v_in);
   vmo_packed_args a = packed_args(q, k, v, q_off, k_off, sm_scale, causal);
   const Tensor o = out ? *out : empty_rows(q);
@@ -716,6 +721,7 @@ std::tuple<Tensor, Tensor, Tensor> packed_bwd(const Tensor& q_in, const Tensor& 
 void cache_checks(const Tensor& x, const Tensor& k_pages, const Tensor& v_pages) {
   require(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), "k_pages and v_pages are (pages, heads, page tokens, D)");
   like(x, {&k_pages, &v_pages});
+  sixteen_bits(x);
 }
 
 Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
@@ -734,6 +740,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
     writable(*out, "vmonarch_amd: out needs 16-byte aligned rows with contiguous features");
   }
   const OnGpuOf device(q_in);
+  if (out) written(*out);
   const Tensor q = readable(q_in), o = out ? *out : at::empty(q_in.sizes(), q_in.options());
   vmo_paged_args a{};
   a.dtype = dtype_code(q);
@@ -758,7 +765,6 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
 void append_pages(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
                   const Tensor& lengths, const OptT& offsets) {
   require(k_in.dim() == 3 && k_in.sizes() == v_in.sizes(), "k and v are (heads, tokens, D), of one shape");
-  dtype_code(k_in);
   like(k_in, v_in);
   cache_checks(k_in, k_pages, v_pages);
   require(k_in.size(0) == k_pages.size(1) && k_in.size(2) == k_pages.size(3), "k and v have the cache's heads and head dim");
@@ -773,6 +779,7 @@ void append_pages(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages,
   }
   for (const Tensor* t : {&k_pages, &v_pages}) writable(*t, "vmonarch_amd: pages need 16-byte aligned rows with contiguous features");
   const OnGpuOf device(k_in);
+  for (const Tensor* t : {&k_pages, &v_pages}) written(*t);
   const Tensor k = readable(k_in), v = readable(v_in);
   vmo_append_args a{};
   a.sequences = size32(lengths.size(0)); a.tokens = size32(k.size(1)); a.kv_heads = size32(k.size(0)); a.d = size32(k.size(2));
@@ -788,12 +795,13 @@ void append_pages(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages,
 void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const std::vector<int64_t>& src, const std::vector<int64_t>& dst) {
   require((k_pages.dim() == 4 || k_pages.dim() == 5) && v_pages.sizes() == k_pages.sizes(),
           "k_pages and v_pages are (pages, heads, page tokens, D), or (layers, pages, ..)");
-  require(k_pages.element_size() == 2, "16-bit pages");
+  sixteen_bits(k_pages);
   like(k_pages, v_pages);
   require(k_pages.is_contiguous() && v_pages.is_contiguous(), "contiguous k_pages and v_pages");
   require(src.size() == dst.size(), "as many pages to copy as places to copy them to");
   const int64_t at = k_pages.dim() - 4, pages = k_pages.size(at);
   const OnGpuOf device(k_pages);
+  for (const Tensor* t : {&k_pages, &v_pages}) written(*t);
   std::vector<int32_t> s, d;
   for (size_t i = 0; i < src.size(); ++i) {
     if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages)

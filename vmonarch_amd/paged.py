@@ -86,6 +86,8 @@ class PagedKVCache:
             raise ValueError(f"vmonarch_amd: pages of {page} tokens (powers of two from 8 to 1024)")
         if min(pages, heads, head_dim, layers) < 1:
             raise ValueError("vmonarch_amd: a cache has pages, heads, features and layers")
+        if dtype not in _lib.DTYPES:
+            raise ValueError(f"vmonarch_amd: a cache of {dtype} (bf16 and fp16 are built)")
         shape = (layers, pages, heads, page, head_dim)
         self.k_pages, self.v_pages = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
         self.page = page
