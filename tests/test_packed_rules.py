@@ -236,3 +236,14 @@ def test_compaction_moves_the_held_pages_down(monkeypatch):
     assert c.free_pages == 9
     c.free(twin)
     assert c.free_pages == 12 and c.grow([c.open()], [8 * 12])[0].tolist() == [list(range(12))]
+
+
+def test_the_cache_records_no_gradients():
+    from vmonarch_amd import append_pages, copy_pages, paged_attention
+    q, k, pages = x(2, 2, 64), x(2, 2, 64), x(3, 2, 8, 64)
+    table, lens = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    for call in (lambda: paged_attention(q.requires_grad_(), pages, pages, table, lens),
+                 lambda: append_pages(k.requires_grad_(), k, pages, pages, table, lens),
+                 lambda: copy_pages(pages.requires_grad_(), pages, [0], [1])):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call()

@@ -321,3 +321,49 @@ def test_sharp_rows(dtype, scale):
         # (as for whole prompts: logits up to 2^9, fp16 weights' floor)
         bound = u * a + u * want.abs() + 2 ** -13 * a + (n * 2.0 ** -25 * 5 if dtype == torch.float16 else 0)
         assert bool(((o[0].double() - want).abs() <= bound).all())
+
+
+def test_calls_at_once_on_streams_of_their_own():
+    """Two threads, each with its stream, its cache and its steps: results as one after the other; out may be q's memory."""
+    import threading
+    from vmonarch_amd import append_pages, copy_pages, paged_attention
+
+    def steps(seed, stream, results):
+        with torch.no_grad(), torch.cuda.stream(stream):
+            g = torch.Generator().manual_seed(seed)
+            k, v, table, lens, _ = cache(g, [100 * seed, 3000, 5], 2, 128, 16, torch.bfloat16)
+            width = torch.full((3, 2), k.shape[0] - 1, dtype=torch.int32, device=DEV)
+            for i in range(10):
+                kn, vn, q = (torch.randn(n, 3, 128, generator=g).bfloat16().to(DEV) for n in (2, 2, 8))
+                q = q.transpose(0, 1).contiguous()
+                lens = torch.clamp(lens + 1, max=3008)
+                append_pages(kn, vn, k, v, torch.cat([table, width], 1), lens)
+                copy_pages(k, v, [0], [k.shape[0] - 2])
+                assert paged_attention(q, k, v, torch.cat([table, width], 1), lens, out=q) is q
+                results.append(q)
+            stream.synchronize()
+
+    alone, beside = [[], []], [[], []]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for j in range(2):
+        steps(j + 2, streams[j], alone[j])
+    threads = [threading.Thread(target=steps, args=(j + 2, streams[j], beside[j])) for j in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(alone, beside):
+        assert len(b) == 10
+        for x, y in zip(a, b):
+            assert not bool(torch.isnan(x.float()).all()) and torch.equal(torch.nan_to_num(x), torch.nan_to_num(y))
+
+
+@pytest.mark.parametrize("page", [8, 512])
+def test_scale_zero_is_the_mean(page):
+    from vmonarch_amd import paged_attention
+    g = torch.Generator().manual_seed(41)
+    k, v, table, lens, rows = cache(g, [77, 1, 2000], 2, 64, page, torch.float16)
+    q = torch.randn(3, 6, 64, generator=g).half().to(DEV)
+    o = paged_attention(q, k, v, table, lens, sm_scale=0.0)
+    for b in range(3):
+        assert_within(o[b], want_one(q[b], rows[b], 0.0, torch.float16), f"sequence {b}")

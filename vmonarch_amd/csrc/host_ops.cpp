@@ -801,7 +801,6 @@ void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const std::vector<
   require(src.size() == dst.size(), "as many pages to copy as places to copy them to");
   const int64_t at = k_pages.dim() - 4, pages = k_pages.size(at);
   const OnGpuOf device(k_pages);
-  for (const Tensor* t : {&k_pages, &v_pages}) written(*t);
   std::vector<int32_t> s, d;
   for (size_t i = 0; i < src.size(); ++i) {
     if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages)
@@ -809,6 +808,7 @@ void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const std::vector<
     s.push_back((int32_t)src[i]);
     d.push_back((int32_t)dst[i]);
   }
+  for (const Tensor* t : {&k_pages, &v_pages}) written(*t);
   vmo_copy_args a{};
   a.layers = size32(at ? k_pages.size(0) : 1); a.pages = size32(pages); a.pairs = size32((int64_t)s.size());
   a.k = k_pages.data_ptr(); a.v = v_pages.data_ptr();

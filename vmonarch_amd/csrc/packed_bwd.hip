@@ -12,7 +12,7 @@
 // Stages that a wave does not see at all are skipped, those on the diagonal (or at a sequence's end) masked.
 // P and dS are rounded to the 16-bit type as operands, the gradients once at the end.  delta takes o as it was before its
 // rounding, from the forward's o and the rounding's error beside it: with the rounded o alone, delta's error was a third of
-// what the roundings of dS and of the gradients give (fp16, dq and dk: 1.52 times the error of one rounding, @@ so).
+// what the roundings of dS and of the gradients give (fp16, dq and dk: 1.52 times the error of one rounding, 1.43 so).
 #include "packed.h"
 
 namespace vmo {
