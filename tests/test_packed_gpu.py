@@ -37,11 +37,14 @@ CASES = [
     ([40, 129, 9], [200, 65, 0], 2, 2, 128, "bf16", "hnd", False),
     ([0, 0], None, 2, 1, 64, "bf16", "hnd", True),
     ([5] * 70 + [150], None, 2, 1, 64, "f16", "nhd", True),             # more sequences than lanes
-    ([3000], None, 2, 1, 64, "f16", "nhd", True),                       # two key groups
+    ([3000], None, 2, 1, 64, "f16", "nhd", True),
     ([2000, 1300], None, 2, 2, 128, "bf16", "hnd", False),
     ([7000], None, 1, 1, 64, "bf16", "hnd", True),                      # heavy tiles in parts
     ([6500, 77], [7100, 77], 2, 2, 128, "bf16", "nhd", True),
     ([6200], None, 2, 1, 128, "f16", "hnd", False),
+    ([9, 0, 140] * 40 + [4100] + [1] * 9, None, 2, 1, 64, "bf16", "nhd", True),   # both
+    ([3, 200] * 50, [130, 0] * 50, 6, 2, 128, "f16", "hnd", True),
+    ([1, 0, 17] * 300, None, 3, 3, 64, "f16", "nhd", False),
 ]
 
 
@@ -185,11 +188,12 @@ def test_offsets_that_lead_outside_are_cut():
         assert torch.isnan(b[:, :200].float()).all() and torch.isnan(b[:, 400:].float()).all()
 
 
-def test_replays_with_other_lengths_from_a_graph():
+@pytest.mark.parametrize("more", [0, 100])   # sequences of no token behind them
+def test_replays_with_other_lengths_from_a_graph(more):
     from vmonarch_amd import packed_attention
     g = torch.Generator().manual_seed(6)
     q, k, v = tensor(g, 4, 500, 128, torch.bfloat16, "nhd"), *(tensor(g, 2, 500, 128, torch.bfloat16, "nhd") for _ in range(2))
-    grad, off = tensor(g, 4, 500, 128, torch.bfloat16, "nhd"), offsets([100, 300, 50])
+    grad, off = tensor(g, 4, 500, 128, torch.bfloat16, "nhd"), offsets([100, 300, 50] + [0] * more)
     leaves = [t.requires_grad_() for t in (q, k, v)]
 
     def step():
@@ -206,7 +210,7 @@ def test_replays_with_other_lengths_from_a_graph():
     with torch.cuda.graph(graph):
         got = step()
     for lengths in ([100, 300, 50], [1, 2, 3], [0, 499, 0], [250, 125, 125]):
-        off.copy_(offsets(lengths))
+        off.copy_(offsets(lengths + [0] * more))
         with torch.no_grad():
             q.copy_(q.roll(1, 1))
         want = [t.detach().clone() for t in step()]

@@ -29,6 +29,9 @@ struct PackedParams {
   float *part, *part2;                     // parts of split tiles: (slots, 128, D) fp32 sums; the forward's m and l (.., 2), or dv's
   float *sum, *sum2;                       // splits > 1: dk's and dv's (splits, kv_heads, tk, D) fp32
   i32x4* records;                          // of the first kPackedParts workgroups: first row, rows, part and parts of its tile
+  i32x4* plan;                             // two of each `idx` (packed_plan): its tile; null: the workgroups find theirs
+  int blocks, per;                         // a launch's workgroups: `blocks` times the `per` of one tile
+  uint32_t per_rcp;                        // (2^32 - 1) / per
   int splits;                              // dk / dv: workgroups that share a key tile, each with group / splits of the heads
   int split_least;                         // tiles of up to so many units are never split (0: no tile is)
   float c, sm_scale;                       // c = sm_scale log2 e
@@ -104,6 +107,7 @@ struct PackedSplit {
   }
   // parts of a sequence's tiles that have at least the work `level`
   __device__ __forceinline__ int count(const PackedTiles& t, int level) const {
+    if (most == 1) return packed_count(t, level);
     int c = 0;
     for (int P = 1; P <= most; ++P) c += P * above(t, P, max(level, 1) - 1);
     if (level <= 0) c += t.tiles - packed_count(t, 1);   // tiles without work
@@ -124,17 +128,28 @@ struct PackedTile {
   int part, parts;
   int which, spare;   // of no tile: the spare workgroup's number, and how many there are
 };
-constexpr int kPackedSeqBytes = 16;   // LDS of a sequence while a workgroup finds its tile
+constexpr int kPackedSeqBytes = 16;   // LDS of a sequence while a wave finds its tile
+constexpr int kPackedFew = 64;        // up to so many sequences a workgroup finds its own tile: one a lane
+
+// Workgroup x is the pos-th of the `per` of part idx.
+struct PackedPlace { int idx, pos; };
+__device__ __forceinline__ PackedPlace packed_place(const PackedParams& p, uint32_t x) {
+  uint32_t q = __umulhi(x, p.per_rcp), r = x - q * (uint32_t)p.per;   // (q or one less than it)
+  if (r >= (uint32_t)p.per) {
+    ++q;
+    r -= p.per;
+  }
+  return PackedPlace{(int)q, (int)r};
+}
 
 // The idx-th part over all sequences' tiles, heaviest tiles first (a tile's time is its keys, or queries: with the heavy ones
-// first the chip's last round is made of light ones); `heads` workgroups take each.  The largest level whose parts and those
+// first the chip's last round is made of light ones); p.per workgroups take each.  The largest level whose parts and those
 // above are more than idx is found by bisection over per-sequence counts, from rows and keys that lie in LDS (free again
-// after the call) where there are more than 64; a level holds the sequences in order.  Every wave does the same.
-template <bool KEYS>
-__device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int idx, int blocks, int heads, VMO_LDS int* lds) {
+// after the call) if MANY, in the lanes else; a level holds the sequences in order.  Every wave of a workgroup calls it.
+template <bool KEYS, bool MANY>
+__device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int idx, VMO_LDS int* lds) {
   const int lane = threadIdx.x & 63;
-  const bool few = p.n <= 64;   // one a lane: each wave reads them itself
-  if (!few) {
+  if constexpr (MANY) {
     for (int s = threadIdx.x; s < p.n; s += (int)blockDim.x) {
       const PackedSeq q = packed_seq(p, s);
       *(VMO_LDS i32x4*)(lds + 4 * s) = i32x4{q.qb, q.nq, q.kb, q.nk};
@@ -146,75 +161,118 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
     return PackedSeq{x[0], x[1], x[2], x[3]};
   };
   PackedSeq mine{0, 0, 0, 0};
-  if (lane < p.n) mine = few ? packed_seq(p, lane) : seq(lane);
+  if (lane < p.n) mine = MANY ? seq(lane) : packed_seq(p, lane);
   const PackedTiles first = packed_tiles<KEYS>(p, mine);
   int best = first.tiles > 0 ? min(first.top, first.cap) : 0;
   float work = packed_work(first);
-  for (int s = lane + 64; s < p.n; s += 64) {
-    const PackedTiles t = packed_tiles<KEYS>(p, seq(s));
-    best = max(best, t.tiles > 0 ? min(t.top, t.cap) : 0);
-    work += packed_work(t);
-  }
+  if constexpr (MANY)
+    for (int s = lane + 64; s < p.n; s += 64) {
+      const PackedTiles t = packed_tiles<KEYS>(p, seq(s));
+      best = max(best, t.tiles > 0 ? min(t.top, t.cap) : 0);
+      work += packed_work(t);
+    }
   best = wave_max_i32(best);
   PackedSplit split{max(best, 1), 1};
-  if (p.split_least > 0) {
+  if (p.split_least > 0 && 4 * best >= 5 * p.split_least) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) work += __shfl_xor(work, m);
-    const float mean = work * (float)heads * (1.001f / kPackedSlots);
+    const float mean = work * (float)p.per * (1.001f / kPackedSlots);
     const int S = max(__builtin_amdgcn_readfirstlane((int)ceilf(fminf(1.75f * mean, 1.0e9f))), p.split_least);
     if (4 * best >= 5 * S) split = PackedSplit{S, (best + S - 1) / S};
   }
   auto total = [&](int level) __attribute__((always_inline)) {
     int c = split.count(first, level);
-    for (int s = lane + 64; s < p.n; s += 64) c += split.count(packed_tiles<KEYS>(p, seq(s)), level);
+    if constexpr (MANY)
+      for (int s = lane + 64; s < p.n; s += 64) c += split.count(packed_tiles<KEYS>(p, seq(s)), level);
     return wave_sum_i32(c);
   };
   PackedTile r;
   r.s = PackedSeq{0, 0, 0, 0};
-  const int all = total(0);
-  r.spare = blocks - all;
   r.tile = -1;
   r.part = 0;
   r.parts = 1;
-  r.which = idx - all;
-  if (idx < all) {
-    int lo = 0, hi = min(split.S, best) + 1;   // total(lo) > idx >= total(hi) = 0
+  r.which = 0;
+  r.spare = 1;
+  int lo = 1, above = 0;   // the level, and the parts above it
+  const int busy = total(1);
+  bool found = idx < busy;
+  if (found) {
+    int hi = min(split.S, best) + 1;   // total(lo) > idx >= total(hi) = above
     while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (total(mid) > idx) lo = mid;
-      else hi = mid;
+      const int mid = (lo + hi) >> 1, t = total(mid);
+      if (t > idx) lo = mid;
+      else hi = mid, above = t;
     }
-    int left = idx - total(lo + 1);
-    for (int s0 = 0; s0 < p.n; s0 += 64) {
-      const PackedSeq q = s0 == 0 ? mine : s0 + lane < p.n ? seq(s0 + lane) : PackedSeq{0, 0, 0, 0};
+  } else {   // tiles without work, then none
+    const int all = total(0);
+    lo = 0;
+    above = busy;
+    found = idx < all;
+    r.which = idx - all;
+    r.spare = p.blocks - all;
+  }
+  if (found) {
+    int left = idx - above;
+    for (int s0 = 0; s0 < (MANY ? p.n : 1); s0 += 64) {
+      const PackedSeq q = !MANY || s0 == 0 ? mine : s0 + lane < p.n ? seq(s0 + lane) : PackedSeq{0, 0, 0, 0};
       const PackedTiles t = packed_tiles<KEYS>(p, q);
       const int here = split.count(t, lo) - split.count(t, lo + 1);
       const int upto = wave_scan_i32(here), sum = __builtin_amdgcn_readlane(upto, 63);
       if (left < sum) {
         const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > left));
         left -= __builtin_amdgcn_readlane(upto, who) - __builtin_amdgcn_readlane(here, who);
-        const PackedTiles it{__builtin_amdgcn_readlane(t.tiles, who), __builtin_amdgcn_readlane(t.top, who),
-                             __builtin_amdgcn_readlane(t.cap, who)};
-        int P = 1, u = packed_count(it, 1) + left;   // (a tile without work)
-        if (lo > 0) {
+        r.s = PackedSeq{__builtin_amdgcn_readlane(q.qb, who), __builtin_amdgcn_readlane(q.nq, who),
+                        __builtin_amdgcn_readlane(q.kb, who), __builtin_amdgcn_readlane(q.nk, who)};
+        const PackedTiles it = packed_tiles<KEYS>(p, r.s);
+        int u = packed_count(it, lo + 1) + left;   // of one part
+        if (split.most > 1 && lo > 0) {
+          int P = 1;
           for (; P < split.most; ++P) {
             const int of_p = P * (split.above(it, P, lo - 1) - split.above(it, P, lo));
             if (left < of_p) break;
             left -= of_p;
           }
           u = packed_count(it, min(P * split.S, P * lo) + 1) + left / P;
+          r.parts = P;
+          r.part = left % P;
         }
-        r.s = PackedSeq{__builtin_amdgcn_readlane(q.qb, who), __builtin_amdgcn_readlane(q.nq, who),
-                        __builtin_amdgcn_readlane(q.kb, who), __builtin_amdgcn_readlane(q.nk, who)};
         r.tile = KEYS || !p.causal ? u : it.tiles - 1 - u;
-        r.parts = P;
-        r.part = lo > 0 ? left % P : 0;
         break;
       }
       left -= sum;
     }
   }
-  if (!few) __syncthreads();   // every wave has read the sequences
+  if constexpr (MANY) __syncthreads();   // every wave has read the sequences
+  return r;
+}
+
+// More than kPackedFew sequences: a launch of its own first, a wave an idx, which leaves each one's tile in the workspace.
+// (Each workgroup looking through all of them for itself: 65 sequences of 100 tokens, 64 heads of 64, 97 us against 64 so; 2048
+// of them, 4 heads: 722 against 135.  With few sequences the search, ~1.5 us, is shorter than a launch.)
+template <bool KEYS>
+__global__ __launch_bounds__(64 * kPackedWaves) void packed_plan_kernel(PackedParams p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem_raw[];
+  const int idx = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kPackedWaves + (int)(threadIdx.x >> 6));
+  const PackedTile w = packed_locate<KEYS, true>(p, idx, (VMO_LDS int*)(VMO_LDS char*)smem_raw);
+  if (idx < p.blocks && (threadIdx.x & 63) == 0) {
+    p.plan[2 * idx] = i32x4{w.s.qb, w.s.nq, w.s.kb, w.s.nk};
+    p.plan[2 * idx + 1] = w.tile < 0 ? i32x4{-1, w.which, w.spare, 0} : i32x4{w.tile, w.part, w.parts, 0};
+  }
+}
+// this workgroup's tile
+template <bool KEYS>
+__device__ __forceinline__ PackedTile packed_tile(const PackedParams& p, int idx) {
+  if (!p.plan) return packed_locate<KEYS, false>(p, idx, nullptr);
+  typedef const __attribute__((address_space(4))) i32x4* scalar_rows;
+  const scalar_rows plan = (scalar_rows)(uintptr_t)p.plan;
+  const i32x4 s = plan[2 * idx], t = plan[2 * idx + 1];
+  PackedTile r;
+  r.s = PackedSeq{s[0], s[1], s[2], s[3]};
+  r.tile = t[0];
+  r.part = t[0] < 0 ? 0 : t[1];
+  r.parts = t[0] < 0 ? 1 : t[2];
+  r.which = t[1];
+  r.spare = t[2];
   return r;
 }
 
@@ -323,20 +381,31 @@ __device__ __forceinline__ void masked_product(f32x16 (&acc)[NA], const VMO_LDS 
 // Head of position `pos` among the workgroups of one tile: block b runs on XCD b % 8, so with g = gcd(8, heads) the
 // positions of one residue mod g stay on 8 / g XCDs; they take neighbouring heads, whose keys and values are shared.
 __device__ __forceinline__ int packed_head(int pos, int heads) {
-  const int g = heads & 7 ? (heads & 3 ? (heads & 1 ? 1 : 2) : 4) : 8;
-  return (pos % g) * (heads / g) + pos / g;
+  const int log = __builtin_ctz(heads | 8), g = 1 << log;
+  return (pos & (g - 1)) * (heads >> log) + (pos >> log);
 }
 
-// Workgroups of a launch with `heads` of a tile each: every tile (a partial one a sequence), the parts of split ones, and one
-// spare at least wherever a row is of no sequence.
-inline int64_t packed_grid(int rows, int n, int heads, bool split) {
-  const int64_t tiles = (int64_t)(rows + kPackedTile - 1) / kPackedTile + n;
-  return (tiles + (split ? (kPackedParts + heads - 1) / heads : 0)) * heads;
+// The parts that a launch has workgroups for, `per` each: every tile (a partial one a sequence), the parts of split ones, and
+// one spare at least wherever a row is of no sequence.
+inline int64_t packed_blocks(int rows, int n, int per, bool split) {
+  return (int64_t)(rows + kPackedTile - 1) / kPackedTile + n + (split ? (kPackedParts + per - 1) / per : 0);
 }
 // Whether tiles may be split (`others`: rows of the other side, in all: offsets are on the GPU): the second kernel's launch,
 // 3 us where it finds nothing to add, is spared short batches.
 constexpr int kPackedSplit = 5;
 inline bool packed_splits(int64_t others) { return others > 1536; }
+
+// The shape of a launch, and with many sequences the launch that finds their tiles first.
+template <bool KEYS>
+inline int packed_begin(PackedParams* p, int rows, int per, hipStream_t s) {
+  p->per = per;
+  p->per_rcp = 0xffffffffu / (uint32_t)per;
+  p->blocks = (int)packed_blocks(rows, p->n, per, p->split_least > 0);
+  if (!p->plan) return VMO_OK;
+  hipLaunchKernelGGL((packed_plan_kernel<KEYS>), dim3((unsigned)((p->blocks + kPackedWaves - 1) / kPackedWaves)),
+                     dim3(64 * kPackedWaves), (size_t)p->n * kPackedSeqBytes, s, *p);
+  return launch_status("packed_plan");
+}
 
 int packed_fwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);
 int packed_bwd_launch(const PackedParams& p, bool f16, int d, hipStream_t s);

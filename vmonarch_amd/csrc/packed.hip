@@ -53,17 +53,27 @@ static int packed_prepare(const vmo_packed_args* a, bool bwd, const char* what, 
 // and dv), between them the backward's -delta.
 static int64_t part_floats(int d) { return (int64_t)kPackedParts * kPackedTile * d; }
 constexpr int64_t kRecordFloats = (int64_t)kPackedParts * 4;
-static int64_t fwd_layout(const vmo_packed_args* a) {
-  return packed_splits(a->tk) ? (kRecordFloats + part_floats(a->d) + part_floats(2)) * 4 : 0;
+// the tiles of many sequences, as a launch before finds them
+static int64_t plan_floats(const vmo_packed_args* a, int rows, int per, int others) {
+  return a->n > kPackedFew ? packed_blocks(rows, a->n, per, packed_splits(others)) * 8 : 0;
 }
-struct BwdLayout { int64_t delta, part, sum, bytes; int splits; };   // floats of -delta, of dk's parts and of its shares' sums
+struct FwdLayout { int64_t plan, bytes; };
+static FwdLayout fwd_layout(const vmo_packed_args* a) {
+  FwdLayout l;
+  l.plan = plan_floats(a, a->tq, a->heads, a->tk);
+  l.bytes = (l.plan + (packed_splits(a->tk) ? kRecordFloats + part_floats(a->d) + part_floats(2) : 0)) * 4;
+  return l;
+}
+struct BwdLayout { int64_t plan, delta, part, sum, bytes; int splits; };   // floats of -delta, of dk's parts and of its shares' sums
 static BwdLayout bwd_layout(const vmo_packed_args* a) {
   BwdLayout l;
   l.delta = ((int64_t)a->heads * a->tq + 63) / 64 * 64;
   l.splits = packed_bwd_splits(a->tk, a->kv_heads, a->heads / a->kv_heads);
   l.part = packed_splits(a->tk) || packed_splits(a->tq) ? part_floats(a->d) : 0;
   l.sum = l.splits > 1 ? (int64_t)l.splits * a->kv_heads * a->tk * a->d : 0;
-  l.bytes = (kRecordFloats + l.delta + 2 * l.part + 2 * l.sum) * 4;
+  const int64_t of_q = plan_floats(a, a->tq, a->heads, a->tk), of_k = plan_floats(a, a->tk, a->kv_heads * l.splits, a->tq);
+  l.plan = of_q > of_k ? of_q : of_k;   // (dq's is read before dk's is written)
+  l.bytes = (l.plan + kRecordFloats + l.delta + 2 * l.part + 2 * l.sum) * 4;
   return l;
 }
 static bool sizes_ok(const vmo_packed_args* a) {
@@ -78,7 +88,7 @@ static int workspace_check(const vmo_packed_args* a, int64_t need, const char* w
 
 }  // namespace vmo
 
-extern "C" size_t vmo_packed_fwd_workspace_size(const vmo_packed_args* a) { return vmo::sizes_ok(a) ? (size_t)vmo::fwd_layout(a) : 0; }
+extern "C" size_t vmo_packed_fwd_workspace_size(const vmo_packed_args* a) { return vmo::sizes_ok(a) ? (size_t)vmo::fwd_layout(a).bytes : 0; }
 
 extern "C" int vmo_packed_fwd(const vmo_packed_args* a, void* stream) {
   using namespace vmo;
@@ -86,12 +96,14 @@ extern "C" int vmo_packed_fwd(const vmo_packed_args* a, void* stream) {
   PackedParams p;
   int rc = packed_prepare(a, false, "packed_fwd", &p);
   if (rc != VMO_OK || a->tq == 0) return rc;
-  rc = workspace_check(a, fwd_layout(a), "packed_fwd");
+  const FwdLayout l = fwd_layout(a);
+  rc = workspace_check(a, l.bytes, "packed_fwd");
   if (rc != VMO_OK) return rc;
+  if (l.plan > 0) p.plan = (i32x4*)a->workspace;
   if (packed_splits(a->tk)) {
     p.split_least = kPackedSplit;
-    p.records = (i32x4*)a->workspace;
-    p.part = (float*)a->workspace + kRecordFloats;
+    p.records = (i32x4*)((float*)a->workspace + l.plan);
+    p.part = (float*)p.records + kRecordFloats;
     p.part2 = p.part + part_floats(a->d);
   }
   return packed_fwd_launch(p, a->dtype == VMO_DTYPE_F16, a->d, (hipStream_t)stream);
@@ -111,8 +123,9 @@ extern "C" int vmo_packed_bwd(const vmo_packed_args* a, void* stream) {
   rc = workspace_check(a, l.bytes, "packed_bwd");
   if (rc != VMO_OK) return rc;
   p.splits = l.splits;
-  p.records = (i32x4*)a->workspace;
-  p.neg_delta = (float*)a->workspace + kRecordFloats;
+  if (l.plan > 0) p.plan = (i32x4*)a->workspace;
+  p.records = (i32x4*)((float*)a->workspace + l.plan);
+  p.neg_delta = (float*)p.records + kRecordFloats;
   p.part = p.neg_delta + l.delta;
   p.part2 = p.part + l.part;
   p.sum = p.part2 + l.part;

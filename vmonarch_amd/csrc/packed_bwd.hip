@@ -22,7 +22,7 @@ constexpr int kKvQueries = 32;   // queries of a dk / dv stage
 
 template <int D> constexpr int packed_dq_lds() {
   constexpr int ring = 2 * kDqKeys * D * 2 * 2;
-  constexpr int least = kPackedWaves * kEpiPatchBytes > kPackedSeqBytes * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : kPackedSeqBytes * kPackedMaxSeqs;
+  constexpr int least = kPackedWaves * kEpiPatchBytes;
   return ring > least ? ring : least;
 }
 // V's 128 rows in LDS at D = 128 (in registers they would spill)
@@ -30,7 +30,7 @@ template <int D> constexpr bool packed_v_in_lds() { return D >= 128; }
 template <int D> constexpr int packed_kv_stage() { return kKvQueries * D * 2 * 2 + 512; }
 template <int D> constexpr int packed_kv_lds() {
   constexpr int ring = 2 * packed_kv_stage<D>() + (packed_v_in_lds<D>() ? kPackedTile * D * 2 : 0);
-  constexpr int least = kPackedWaves * kEpiPatchBytes > kPackedSeqBytes * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : kPackedSeqBytes * kPackedMaxSeqs;
+  constexpr int least = kPackedWaves * kEpiPatchBytes;
   return ring > least ? ring : least;
 }
 
@@ -52,8 +52,9 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
   const uint32_t smem_u32 = (uint32_t)(uintptr_t)smem;
   auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
 
-  const int head = uni(packed_head((int)blockIdx.x % p.heads, p.heads));
-  const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, p.heads, (VMO_LDS int*)smem);
+  const PackedPlace place = packed_place(p, blockIdx.x);
+  const int head = uni(packed_head(place.pos, p.heads));
+  const PackedTile w = packed_tile<false>(p, place.idx);
   packed_record<false>(p, w);
   if (w.tile < 0) {
     packed_zero_rest<T, D>((T*)p.dq + head * p.dq_sh, p.dq_sn, p.q_off, p.n, p.tq, w.which, w.spare);
@@ -205,10 +206,11 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   const uint32_t smem_u32 = (uint32_t)(uintptr_t)smem;
   auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
 
-  const int shares = p.kv_heads * p.splits;   // workgroups of one key tile (a share stays on its XCDs, so its heads' rows do)
-  const int hs = uni(packed_head((int)blockIdx.x % shares, shares));
+  // kv_heads x splits workgroups of one key tile (a share stays on its XCDs, so its heads' rows do)
+  const PackedPlace place = packed_place(p, blockIdx.x);
+  const int hs = uni(packed_head(place.pos, p.per));
   const int kvh = hs / p.splits, split = hs % p.splits;
-  const PackedTile w = packed_locate<true>(p, (int)blockIdx.x / shares, (int)gridDim.x / shares, shares, (VMO_LDS int*)smem);
+  const PackedTile w = packed_tile<true>(p, place.idx);
   packed_record<true>(p, w);
   if (w.tile < 0) {
     if (p.splits == 1) {
@@ -409,7 +411,7 @@ __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams p) {
   constexpr int TPR = D / 4;
   const i32x4 rec = p.records[blockIdx.x];   // first row, rows, part, parts
   if (rec[3] <= 1) return;
-  const int shares = KEYS ? p.kv_heads * p.splits : p.heads, hs = packed_head((int)blockIdx.x % shares, shares), parts = rec[3];
+  const int shares = p.per, hs = packed_head(packed_place(p, blockIdx.x).pos, shares), parts = rec[3];
   const int head = KEYS ? hs / p.splits : hs, d4 = (threadIdx.x % TPR) * 4;
   const int64_t slot0 = (int)blockIdx.x - rec[2] * shares;
   for (int r = rec[2] * rec[1] / parts + threadIdx.x / TPR; r < (rec[2] + 1) * rec[1] / parts; r += 256 / TPR) {
@@ -497,8 +499,9 @@ static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   int rc = VMO_OK;
   if (p.tq > 0) {
     p.split_least = packed_splits(p.tk) ? kPackedSplit : 0;
-    const int64_t grid = packed_grid(p.tq, p.n, p.heads, p.split_least > 0);
-    hipLaunchKernelGGL((packed_bwd_dq_kernel<F16, D>), dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_Q, s, p);
+    rc = packed_begin<false>(&p, p.tq, p.heads, s);
+    if (rc != VMO_OK) return rc;
+    hipLaunchKernelGGL((packed_bwd_dq_kernel<F16, D>), dim3((unsigned)(p.blocks * p.per)), dim3(64 * kPackedWaves), LDS_Q, s, p);
     rc = launch_status("packed_bwd_dq");
     if (rc == VMO_OK && p.split_least > 0) rc = join(packed_bwd_join_kernel<F16, D, false>);
     if (rc != VMO_OK) return rc;
@@ -509,8 +512,9 @@ static int launch_packed_bwd(PackedParams p, hipStream_t s) {
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_KV) != hipSuccess)
     return set_error(VMO_ERR_LAUNCH, "packed_bwd: cannot raise the LDS limit to %d bytes", LDS_KV);
   p.split_least = packed_splits(p.tq) ? kPackedSplit : 0;
-  const int64_t grid = packed_grid(p.tk, p.n, p.kv_heads * p.splits, p.split_least > 0);
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS_KV, s, p);
+  rc = packed_begin<true>(&p, p.tk, p.kv_heads * p.splits, s);
+  if (rc != VMO_OK) return rc;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(p.blocks * p.per)), dim3(64 * kPackedWaves), LDS_KV, s, p);
   rc = launch_status("packed_bwd_dkdv");
   if (rc != VMO_OK) return rc;
   if (p.split_least > 0) rc = join(packed_bwd_join_kernel<F16, D, true>);

@@ -27,7 +27,7 @@ constexpr float kNoMax = -3.0e38f;    // m of a row that has seen no key
 template <int D> constexpr int packed_stage_bytes() { return kFwdBN * D * 2 * 2; }
 template <int D> constexpr int packed_fwd_lds() {
   constexpr int ring = fwd_slots(packed_stage_bytes<D>()) * packed_stage_bytes<D>();
-  constexpr int least = kPackedWaves * kEpiPatchBytes > kPackedSeqBytes * kPackedMaxSeqs ? kPackedWaves * kEpiPatchBytes : kPackedSeqBytes * kPackedMaxSeqs;
+  constexpr int least = kPackedWaves * kEpiPatchBytes;
   return ring > least ? ring : least;
 }
 
@@ -44,8 +44,9 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
   VMO_LDS char* smem = (VMO_LDS char*)smem_raw;
   auto uni = [](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(x); };
 
-  const int head = uni(packed_head((int)blockIdx.x % p.heads, p.heads));
-  const PackedTile w = packed_locate<false>(p, (int)blockIdx.x / p.heads, (int)gridDim.x / p.heads, p.heads, (VMO_LDS int*)smem);
+  const PackedPlace place = packed_place(p, blockIdx.x);
+  const int head = uni(packed_head(place.pos, p.heads));
+  const PackedTile w = packed_tile<false>(p, place.idx);
   packed_record<false>(p, w);
   if (w.tile < 0) {
     if (p.zero_rest)
@@ -318,7 +319,7 @@ __global__ __launch_bounds__(256) void packed_fwd_join_kernel(PackedParams p) {
   constexpr int TPR = D / 4;
   const i32x4 rec = p.records[blockIdx.x];   // first row, rows, part, parts
   if (rec[3] <= 1) return;
-  const int head = packed_head((int)blockIdx.x % p.heads, p.heads), d4 = (threadIdx.x % TPR) * 4, parts = rec[3];
+  const int head = packed_head(packed_place(p, blockIdx.x).pos, p.heads), d4 = (threadIdx.x % TPR) * 4, parts = rec[3];
   const int slot0 = (int)blockIdx.x - rec[2] * p.heads;
   for (int r = rec[2] * rec[1] / parts + threadIdx.x / TPR; r < (rec[2] + 1) * rec[1] / parts; r += 256 / TPR) {
     float m = kNoMax, l = 0.f;
@@ -350,12 +351,13 @@ __global__ __launch_bounds__(256) void packed_fwd_join_kernel(PackedParams p) {
 }
 
 template <bool F16, int D>
-static int launch_packed_fwd(const PackedParams& p, hipStream_t s) {
+static int launch_packed_fwd(PackedParams p, hipStream_t s) {
   constexpr int LDS = packed_fwd_lds<D>();
   static_assert(LDS <= 65536, "LDS within the default limit");
-  const int64_t grid = packed_grid(p.tq, p.n, p.heads, p.split_least > 0);
-  hipLaunchKernelGGL((packed_fwd_kernel<F16, D>), dim3((unsigned)grid), dim3(64 * kPackedWaves), LDS, s, p);
-  const int rc = launch_status("packed_fwd");
+  int rc = packed_begin<false>(&p, p.tq, p.heads, s);
+  if (rc != VMO_OK) return rc;
+  hipLaunchKernelGGL((packed_fwd_kernel<F16, D>), dim3((unsigned)(p.blocks * p.per)), dim3(64 * kPackedWaves), LDS, s, p);
+  rc = launch_status("packed_fwd");
   if (rc != VMO_OK || p.split_least == 0) return rc;
   hipLaunchKernelGGL((packed_fwd_join_kernel<F16, D>), dim3(kPackedParts), dim3(256), 0, s, p);
   return launch_status("packed_fwd_join");
