@@ -606,6 +606,12 @@ void writable(const Tensor& t, const char* msg) {
 }
 // a tensor that a call writes in place: autograd learns of it as of torch's own in-place operations
 void written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+// the cache's operators have no backward: a call that would be recorded is refused
+void not_recorded(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    if (t->requires_grad()) throw std::runtime_error(std::string("vmonarch_amd: ") + what + " is not differentiable: call it under torch.no_grad()");
+}
 void sixteen_bits(const Tensor& t) { require(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, "bf16 or fp16 tensors"); }
 vmo_view rows_view(const Tensor& t) { return vmo_view{t.data_ptr(), 0, t.stride(0), t.stride(1)}; }   // (heads, tokens, D)
 vmo_view pages_view(const Tensor& t) { return vmo_view{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
@@ -726,6 +732,7 @@ void cache_checks(const Tensor& x, const Tensor& k_pages, const Tensor& v_pages)
 
 Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
                        double sm_scale, const OptT& out) {
+  not_recorded("paged_attention", {&q_in, &k_pages, &v_pages});
   require(q_in.dim() == 3, "q is (sequences, heads, D)");
   cache_checks(q_in, k_pages, v_pages);
   require(q_in.size(2) == k_pages.size(3), "q has the cache's head dim");
@@ -764,6 +771,7 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_pages, const Tensor& 
 
 void append_pages(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
                   const Tensor& lengths, const OptT& offsets) {
+  not_recorded("append_pages", {&k_in, &v_in, &k_pages, &v_pages});
   require(k_in.dim() == 3 && k_in.sizes() == v_in.sizes(), "k and v are (heads, tokens, D), of one shape");
   like(k_in, v_in);
   cache_checks(k_in, k_pages, v_pages);
@@ -793,6 +801,7 @@ void append_pages(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages,
 }
 
 void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const std::vector<int64_t>& src, const std::vector<int64_t>& dst) {
+  not_recorded("copy_pages", {&k_pages, &v_pages});
   require((k_pages.dim() == 4 || k_pages.dim() == 5) && v_pages.sizes() == k_pages.sizes(),
           "k_pages and v_pages are (pages, heads, page tokens, D), or (layers, pages, ..)");
   sixteen_bits(k_pages);

@@ -9,12 +9,6 @@ import heapq
 import torch
 
 from . import _lib
-from .kernel import _recorded
-
-
-def _not_recorded(what, *tensors):
-    if _recorded(*tensors):
-        raise RuntimeError(f"vmonarch_amd: {what} is not differentiable: call it under torch.no_grad()")
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, sm_scale=None, out=None):
@@ -36,7 +30,6 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, sm_scale=None, out
     page number outside the cache, or a length beyond W pages, is not followed: that sequence's rows are NaN.  Not
     differentiable: where gradients are recorded the call is refused, as those below are.
     """
-    _not_recorded("paged_attention", q, k_pages, v_pages)
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
     return _lib.host().paged_attention(q, k_pages, v_pages, page_table, lengths, sm_scale, out)
@@ -56,7 +49,6 @@ def append_pages(k, v, k_pages, v_pages, page_table, lengths, offsets=None):
     A row of no sequence, or one whose place or page number is outside the cache, is left out.  Sequences must not share
     the pages that they are writing to (PagedKVCache copies such a page first).
     """
-    _not_recorded("append_pages", k, v, k_pages, v_pages)
     _lib.host().append_pages(k, v, k_pages, v_pages, page_table, lengths, offsets)
 
 
@@ -66,7 +58,6 @@ def copy_pages(k_pages, v_pages, src, dst):
     same pages of every layer.  src and dst are sequences of numbers on the host, which the launch carries (a captured
     graph repeats these very copies).  A page that is written twice, or written and read, is refused.
     """
-    _not_recorded("copy_pages", k_pages, v_pages)
     _lib.host().copy_pages(k_pages, v_pages, src, dst)
 
 
