@@ -98,6 +98,7 @@ __device__ __forceinline__ int packed_count(const PackedTiles& t, int level) {
 // 2 kPackedSlots / 1.75 workgroups.  A part's fp32 sums go to slot = workgroup number; a second kernel adds them.
 constexpr int kPackedSlots = 512;
 constexpr int kPackedParts = 2 * kPackedSlots + 128;
+constexpr int kJoinRows = 4;   // rows that a lane of an adding kernel has under way
 struct PackedSplit {
   int S, most;   // units a part has at most; parts a tile has at most
   __device__ __forceinline__ int parts(int L) const { return L > S ? (L + S - 1) / S : 1; }

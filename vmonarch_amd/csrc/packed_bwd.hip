@@ -403,43 +403,52 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
 }
 
 // dq, or dk and dv, of split tiles from their parts, in the parts' order: the workgroup of part k takes its share of the
-// tile's rows, D / 4 lanes a row.
+// tile's rows, D / 4 lanes a row, kJoinRows of them at a time.
 template <bool F16, int D, bool KEYS>
 __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams p) {
   using T = typename Elem<F16>::T;
   using V4 = typename Elem<F16>::V4;
-  constexpr int TPR = D / 4;
+  constexpr int TPR = D / 4, STEP = 256 / TPR;
   const i32x4 rec = p.records[blockIdx.x];   // first row, rows, part, parts
   if (rec[3] <= 1) return;
   const int shares = p.per, hs = packed_head(packed_place(p, blockIdx.x).pos, shares), parts = rec[3];
   const int head = KEYS ? hs / p.splits : hs, d4 = (threadIdx.x % TPR) * 4;
   const int64_t slot0 = (int)blockIdx.x - rec[2] * shares;
-  for (int r = rec[2] * rec[1] / parts + threadIdx.x / TPR; r < (rec[2] + 1) * rec[1] / parts; r += 256 / TPR) {
-    f32x4 a = f32x4{}, b = f32x4{};
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const int64_t at = ((slot0 + i * shares) * kPackedTile + r) * D + d4;
-      a += *(const f32x4*)(p.part + at);
-      if constexpr (KEYS) b += *(const f32x4*)(p.part2 + at);
-    }
-    const int64_t tok = rec[0] + r;
-    if (KEYS && p.splits > 1) {   // a share's sums: packed_bwd_sum adds the shares
-      const int64_t at = ((int64_t)(hs % p.splits * p.kv_heads + head) * p.tk + tok) * D + d4;
-      *(f32x4*)(p.sum + at) = a;
-      *(f32x4*)(p.sum2 + at) = b;
-      continue;
-    }
-    V4 x, y;
+  const int end = (rec[2] + 1) * rec[1] / parts;
+  for (int r0 = rec[2] * rec[1] / parts + threadIdx.x / TPR; r0 < end; r0 += kJoinRows * STEP) {
+    f32x4 a[kJoinRows], b[kJoinRows];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = to_elem<T>(a[e]);
-      y[e] = to_elem<T>(b[e]);
-    }
-    if constexpr (KEYS) {
-      *(V4*)((T*)p.dk + (int64_t)head * p.dk_sh + tok * p.dk_sn + d4) = x;
-      *(V4*)((T*)p.dv + (int64_t)head * p.dv_sh + tok * p.dv_sn + d4) = y;
-    } else {
-      *(V4*)((T*)p.dq + (int64_t)head * p.dq_sh + tok * p.dq_sn + d4) = x;
+    for (int j = 0; j < kJoinRows; ++j) a[j] = b[j] = f32x4{};
+#pragma unroll 2
+    for (int i = 0; i < parts; ++i)
+#pragma unroll
+      for (int j = 0; j < kJoinRows; ++j) {
+        const int64_t at = ((slot0 + i * shares) * kPackedTile + min(r0 + j * STEP, end - 1)) * D + d4;
+        a[j] += *(const f32x4*)(p.part + at);
+        if constexpr (KEYS) b[j] += *(const f32x4*)(p.part2 + at);
+      }
+#pragma unroll
+    for (int j = 0; j < kJoinRows; ++j) {
+      if (r0 + j * STEP >= end) break;
+      const int64_t tok = rec[0] + r0 + j * STEP;
+      if (KEYS && p.splits > 1) {   // a share's sums: packed_bwd_sum adds the shares
+        const int64_t at = ((int64_t)(hs % p.splits * p.kv_heads + head) * p.tk + tok) * D + d4;
+        *(f32x4*)(p.sum + at) = a[j];
+        *(f32x4*)(p.sum2 + at) = b[j];
+        continue;
+      }
+      V4 x, y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = to_elem<T>(a[j][e]);
+        y[e] = to_elem<T>(b[j][e]);
+      }
+      if constexpr (KEYS) {
+        *(V4*)((T*)p.dk + (int64_t)head * p.dk_sh + tok * p.dk_sn + d4) = x;
+        *(V4*)((T*)p.dv + (int64_t)head * p.dv_sh + tok * p.dv_sn + d4) = y;
+      } else {
+        *(V4*)((T*)p.dq + (int64_t)head * p.dq_sh + tok * p.dq_sn + d4) = x;
+      }
     }
   }
 }
@@ -451,27 +460,29 @@ __global__ __launch_bounds__(256) void packed_bwd_sum_kernel(PackedParams p) {
   using T = typename Elem<F16>::T;
   using V4 = typename Elem<F16>::V4;
   constexpr int TPR = D / 4;
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t rows = (int64_t)p.kv_heads * p.tk, r = gid / TPR;
-  const int c4 = (int)(gid % TPR) * 4;
-  if (r >= rows) return;
-  const int kvh = (int)(r / p.tk), tok = (int)(r % p.tk);
-  f32x4 a = f32x4{}, b = f32x4{};
-  if (tok >= min(max(p.k_off[0], 0), p.tk) && tok < min(max(p.k_off[p.n], 0), p.tk))
+  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)p.kv_heads * p.tk;
+  const int tok = (int)(gid / TPR), c4 = (int)(gid % TPR) * 4;
+  if (tok >= p.tk) return;
+  const int first = p.k_off[0], last = p.k_off[p.n];
+  const bool held = tok >= min(max(first, 0), p.tk) && tok < min(max(last, 0), p.tk);
+  for (int kvh = blockIdx.y; kvh < p.kv_heads; kvh += (int)gridDim.y) {
+    const int64_t r = (int64_t)kvh * p.tk + tok;
+    f32x4 a = f32x4{}, b = f32x4{};
 #pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
+    for (int s = 0; s < p.splits; ++s) {   // (of a row of no sequence: whatever lies there, not used)
       const int64_t at = (s * rows + r) * D + c4;
       a += *(const f32x4*)(p.sum + at);
       b += *(const f32x4*)(p.sum2 + at);
     }
-  V4 x, y;
+    V4 x, y;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[e] = to_elem<T>(a[e]);
-    y[e] = to_elem<T>(b[e]);
+    for (int e = 0; e < 4; ++e) {
+      x[e] = to_elem<T>(held ? a[e] : 0.f);
+      y[e] = to_elem<T>(held ? b[e] : 0.f);
+    }
+    *(V4*)((T*)p.dk + (int64_t)kvh * p.dk_sh + (int64_t)tok * p.dk_sn + c4) = x;
+    *(V4*)((T*)p.dv + (int64_t)kvh * p.dv_sh + (int64_t)tok * p.dv_sn + c4) = y;
   }
-  *(V4*)((T*)p.dk + (int64_t)kvh * p.dk_sh + (int64_t)tok * p.dk_sn + c4) = x;
-  *(V4*)((T*)p.dv + (int64_t)kvh * p.dv_sh + (int64_t)tok * p.dv_sn + c4) = y;
 }
 
 // Workgroups that share a key tile, each with some of the group's heads: as many as divide the group and bring the launch to
@@ -519,8 +530,9 @@ static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   if (rc != VMO_OK) return rc;
   if (p.split_least > 0) rc = join(packed_bwd_join_kernel<F16, D, true>);
   if (rc != VMO_OK || p.splits == 1) return rc;
-  const int64_t threads = (int64_t)p.kv_heads * p.tk * (D / 4);
-  hipLaunchKernelGGL((packed_bwd_sum_kernel<F16, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
+  const int64_t threads = (int64_t)p.tk * (D / 4);
+  hipLaunchKernelGGL((packed_bwd_sum_kernel<F16, D>), dim3((unsigned)((threads + 255) / 256), (unsigned)min(p.kv_heads, 65535)),
+                     dim3(256), 0, s, p);
   return launch_status("packed_bwd_sum");
 }
 

@@ -312,41 +312,56 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
     p.lse[(int64_t)head * p.st_sh + qb + q0 + l32] = l_tot == 0.f ? 0.f : m_run + fast_log2(l_tot);
 }
 
-// o (and lse) of split tiles from their parts: the workgroup of part k takes its share of the tile's rows, D / 4 lanes a row.
+// o (and lse) of split tiles from their parts: the workgroup of part k takes its share of the tile's rows, D / 4 lanes a row,
+// kJoinRows of them at a time, whose loads are under way together.
 template <bool F16, int D>
 __global__ __launch_bounds__(256) void packed_fwd_join_kernel(PackedParams p) {
   using T = typename Elem<F16>::T;
-  constexpr int TPR = D / 4;
+  constexpr int TPR = D / 4, STEP = 256 / TPR;
   const i32x4 rec = p.records[blockIdx.x];   // first row, rows, part, parts
   if (rec[3] <= 1) return;
   const int head = packed_head(packed_place(p, blockIdx.x).pos, p.heads), d4 = (threadIdx.x % TPR) * 4, parts = rec[3];
   const int slot0 = (int)blockIdx.x - rec[2] * p.heads;
-  for (int r = rec[2] * rec[1] / parts + threadIdx.x / TPR; r < (rec[2] + 1) * rec[1] / parts; r += 256 / TPR) {
-    float m = kNoMax, l = 0.f;
-    f32x4 acc = f32x4{};
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const int64_t at = (int64_t)(slot0 + i * p.heads) * kPackedTile + r;
-      const float pm = p.part2[2 * at], pl = p.part2[2 * at + 1];
-      const f32x4 y = *(const f32x4*)(p.part + at * D + d4);
-      const float m_new = fmaxf(m, pm), f = fast_exp2(m - m_new), pf = fast_exp2(pm - m_new);
-      m = m_new;
-      l = fmaf(l, f, pl * pf);
+  const int end = (rec[2] + 1) * rec[1] / parts;
+  for (int r0 = rec[2] * rec[1] / parts + threadIdx.x / TPR; r0 < end; r0 += kJoinRows * STEP) {
+    float m[kJoinRows], l[kJoinRows];
+    f32x4 acc[kJoinRows];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(acc[e], f, y[e] * pf);
+    for (int j = 0; j < kJoinRows; ++j) {
+      m[j] = kNoMax;
+      l[j] = 0.f;
+      acc[j] = f32x4{};
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    typename Elem<F16>::V4 y, low;
+#pragma unroll 2
+    for (int i = 0; i < parts; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = acc[e] * inv;
-      y[e] = to_elem<T>(x);
-      low[e] = to_elem<T>(x - (float)y[e]);
+      for (int j = 0; j < kJoinRows; ++j) {
+        const int64_t at = (int64_t)(slot0 + i * p.heads) * kPackedTile + min(r0 + j * STEP, end - 1);
+        const float pm = p.part2[2 * at], pl = p.part2[2 * at + 1];
+        const f32x4 y = *(const f32x4*)(p.part + at * D + d4);
+        const float m_new = fmaxf(m[j], pm), f = fast_exp2(m[j] - m_new), pf = fast_exp2(pm - m_new);
+        m[j] = m_new;
+        l[j] = fmaf(l[j], f, pl * pf);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(acc[j][e], f, y[e] * pf);
+      }
+#pragma unroll
+    for (int j = 0; j < kJoinRows; ++j) {
+      const int r = r0 + j * STEP;
+      if (r >= end) break;
+      const float inv = l[j] == 0.f ? 0.f : 1.0f / l[j];
+      typename Elem<F16>::V4 y, low;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = acc[j][e] * inv;
+        y[e] = to_elem<T>(x);
+        low[e] = to_elem<T>(x - (float)y[e]);
+      }
+      const int64_t tok = rec[0] + r, at = (int64_t)head * p.o_sh + tok * p.o_sn + d4;
+      *(typename Elem<F16>::V4*)((T*)p.out + at) = y;
+      if (p.o_low) *(typename Elem<F16>::V4*)((T*)p.o_low + at) = low;
+      if (p.lse && d4 == 0) p.lse[(int64_t)head * p.st_sh + tok] = l[j] == 0.f ? 0.f : m[j] + fast_log2(l[j]);
     }
-    const int64_t tok = rec[0] + r, at = (int64_t)head * p.o_sh + tok * p.o_sn + d4;
-    *(typename Elem<F16>::V4*)((T*)p.out + at) = y;
-    if (p.o_low) *(typename Elem<F16>::V4*)((T*)p.o_low + at) = low;
-    if (p.lse && d4 == 0) p.lse[(int64_t)head * p.st_sh + tok] = l == 0.f ? 0.f : m + fast_log2(l);
   }
 }
 

@@ -326,14 +326,14 @@ __global__ __launch_bounds__(64) void paged_attention_kernel(PagedParams p) {
 
 // o of a row that several waves hold, one query head a workgroup: the workgroup of the first wave that begins inside it.
 // D / 4 lanes a part, 256 / (D / 4) parts side by side, each group with a running maximum over its own, then the groups in
-// LDS in their order.  Bound by the latency of three reads in a row (starts, starts of the waves behind, parts).
+// LDS in their order.  Bound by the latency of two reads in a row (starts, parts).
 template <bool F16, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   using T = typename Elem<F16>::T;
   constexpr int TPR = D / 4, NG = 256 / TPR;
   __shared__ float sums[NG][D], ml[NG][2];
   const int w = blockIdx.x, in = blockIdx.y, tid = threadIdx.x;
-  const int row = p.starts[w], last = w > 0 ? p.starts[w - 1] : -1;
+  const int row = p.starts[w], last = w > 0 ? p.starts[w - 1] : -1, near = p.starts[min(w + tid, p.waves - 1)];
   if (row < 0 || row == last) return;
   const int X = p.kv_heads * p.blocks, b = row / X, x = row % X, block = x % p.blocks;
   if (in >= min(p.per, p.group - block * p.per)) return;
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedParams p) {
   int more = 0;
   for (bool on = true; on; ) {
     const int v = w + more + tid;
-    const uint64_t out = __builtin_amdgcn_ballot_w64(v >= p.waves || p.starts[min(v, p.waves - 1)] != row);
+    const uint64_t out = __builtin_amdgcn_ballot_w64(v >= p.waves || (more == 0 ? near : p.starts[min(v, p.waves - 1)]) != row);
     if ((tid & 63) == 0) firsts[tid >> 6] = out ? __builtin_ctzll(out) : 64;
     __syncthreads();
 #pragma unroll
