@@ -89,13 +89,15 @@ __device__ __forceinline__ int packed_count(const PackedTiles& t, int level) {
 
 // Heavy tiles are split: one long prompt's last tile sees all its keys, and alone can take longer than the whole launch's mean
 // work.  S is 1.75 times the mean of the chip's kPackedSlots workgroups -- one that has its CU alone runs about that much
-// faster than two that share it, so up to S a tile is no later than the rest -- and `split_least` at least; where the
-// heaviest tile has 1.25 S, those of L > S units are cut into ceil(L / S) parts of equal length.  One prompt of 16384 tokens,
-// 2 heads of 128 over one: 248 -> 168 us; of 8192, 4 heads: 129 -> 97; 4 prompts of 20 to 5000, 4 heads: 85 -> 59; with S the
-// mean itself the parts' own cost shows (8192 tokens, 12 heads: 215 -> 231), and eight waves of two key groups instead, which
-// halve every tile's time, did less (176 and 99 -> 218 and 116).  Parts and whole tiles stand in one order, by their work, so
-// the launch's last round is made of light ones; as no part has less than half of S, all parts are among the first
-// 2 kPackedSlots / 1.75 workgroups.  A part's fp32 sums go to slot = workgroup number; a second kernel adds them.
+// faster than two that share it, so up to S a tile is no later than the rest --, or 6 above 1.25 times the mean where that is
+// less (long prompts, beside whose stages a part's own cost is small), and `split_least` at least; where the heaviest tile has
+// 1.25 S, those of L > S units are cut into ceil(L / S) parts of equal length.  One prompt of 16384 tokens, 2 heads of 128
+// over one: 248 -> 163 us; of 8192, 4 heads: 129 -> 92; 4 prompts of 20 to 5000, 4 heads: 85 -> 55.  Training steps of the
+// first two: 714 -> 677 and 405 -> 396 us against 1.75 times the mean everywhere; 1.25 times everywhere cost short batches (12
+// prompts of 40 to 3900 keys, 12 heads: 75 -> 84 us).  Eight waves of two key groups instead, which halve every tile's time,
+// did less (176 and 99 -> 218 and 116).  Parts and whole tiles stand in one order, by their work, so the launch's last round
+// is made of light ones; as no part has less than half of S, all parts are among the first 2 kPackedSlots / 1.25 workgroups.
+// A part's fp32 sums go to slot = workgroup number; a second kernel adds them.
 constexpr int kPackedSlots = 512;
 constexpr int kPackedParts = 2 * kPackedSlots + 128;
 constexpr int kJoinRows = 4;   // rows that a lane of an adding kernel has under way
@@ -178,7 +180,7 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) work += __shfl_xor(work, m);
     const float mean = work * (float)p.per * (1.001f / kPackedSlots);
-    const int S = max(__builtin_amdgcn_readfirstlane((int)ceilf(fminf(1.75f * mean, 1.0e9f))), p.split_least);
+    const int S = max(__builtin_amdgcn_readfirstlane((int)ceilf(fminf(fminf(1.75f * mean, 1.25f * mean + 6.f), 1.0e9f))), p.split_least);
     if (4 * best >= 5 * S) split = PackedSplit{S, (best + S - 1) / S};
   }
   auto total = [&](int level) __attribute__((always_inline)) {
