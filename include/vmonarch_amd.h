@@ -3,9 +3,9 @@
  *
  * The reference (EricLina/VMonarch) has no C/C++ API: its device code is Triton JIT kernels
  * launched from Python.  Each entry point below replaces one launch site of the reference's
- * Python, keeping the argument meaning; the Python package `vmonarch_amd` (and the alias
- * package `video_monarch_attention`) binds them with ctypes and keeps the reference's Python
- * API unchanged.
+ * Python, keeping the argument meaning, unless it says that it has no counterpart there; the
+ * Python package `vmonarch_amd` (and the alias package `video_monarch_attention`) binds them
+ * with ctypes and keeps the reference's Python API unchanged.
  *
  * Conventions
  *   - Every call is asynchronous on the given HIP stream (a hipStream_t passed as void*,
