@@ -168,6 +168,25 @@ def test_rows_of_no_sequence_and_out():
         assert not bool(t[:, :a].any()) and not bool(t[:, b:].any()) and torch.isfinite(t.float()).all()
 
 
+def test_many_sequences_with_rows_outside():
+    """More sequences than a workgroup looks through itself, rows before the first and behind the last one: zeros there, the
+    rest as without them."""
+    from vmonarch_amd import packed_attention
+    g = torch.Generator().manual_seed(8)
+    lengths, before, behind = [17, 0, 130] * 40 + [1900], 300, 500
+    n = sum(lengths)
+    q, k, v, grad = (tensor(g, h, before + n + behind, 64, torch.bfloat16, "nhd") for h in (4, 2, 2, 4))
+    inner = [t[:, before:before + n] for t in (q, k, v, grad)]
+    want_leaves = [t.detach().requires_grad_() for t in inner[:3]]
+    want = packed_attention(*want_leaves, offsets(lengths))
+    want_grads = torch.autograd.grad(want, want_leaves, inner[3])
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = packed_attention(*leaves, offsets(lengths) + before)
+    for got, x in zip((o, *torch.autograd.grad(o, leaves, grad)), (want, *want_grads)):
+        assert torch.equal(got[:, before:before + n], x)
+        assert not bool(got[:, :before].any()) and not bool(got[:, before + n:].any())
+
+
 def test_offsets_that_lead_outside_are_cut():
     """Nothing outside the tensors is read or written, whatever the offsets hold: the tensors are the middle of larger
     buffers whose edges would show it."""

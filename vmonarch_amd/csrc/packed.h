@@ -35,6 +35,7 @@ struct PackedParams {
   int splits;                              // dk / dv: workgroups that share a key tile, each with group / splits of the heads
   int split_least;                         // tiles of up to so many units are never split (0: no tile is)
   float c, sm_scale;                       // c = sm_scale log2 e
+  float* part_q;                           // the backward's launch: dq's parts (part, part2: dk's and dv's)
 };
 
 // ---- integer sums over a wave (DPP: row shifts, then the rows' last lanes broadcast) --------------------------------

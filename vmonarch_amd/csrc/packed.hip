@@ -49,8 +49,8 @@ static int packed_prepare(const vmo_packed_args* a, bool bwd, const char* what, 
   return VMO_OK;
 }
 
-// Workspaces: the records of split tiles and their parts (the forward's with their m and l, the backward's of dq, then of dk
-// and dv), between them the backward's -delta.
+// Workspaces: the plan of many sequences; the records of split tiles and their parts (the forward's with their m and l, the
+// backward's of dk, dv and dq); the backward's -delta and the sums of its shares.
 static int64_t part_floats(int d) { return (int64_t)kPackedParts * kPackedTile * d; }
 constexpr int64_t kRecordFloats = (int64_t)kPackedParts * 4;
 // the tiles of many sequences, as a launch before finds them
@@ -64,16 +64,17 @@ static FwdLayout fwd_layout(const vmo_packed_args* a) {
   l.bytes = (l.plan + (packed_splits(a->tk) ? kRecordFloats + part_floats(a->d) + part_floats(2) : 0)) * 4;
   return l;
 }
-struct BwdLayout { int64_t plan, delta, part, sum, bytes; int splits; };   // floats of -delta, of dk's parts and of its shares' sums
+struct BwdLayout { int64_t plan, delta, part_q, part, sum, bytes; int splits; };   // floats of -delta, dq's and dk's parts, dk's shares' sums
 static BwdLayout bwd_layout(const vmo_packed_args* a) {
   BwdLayout l;
   l.delta = ((int64_t)a->heads * a->tq + 63) / 64 * 64;
   l.splits = packed_bwd_splits(a->tk, a->kv_heads, a->heads / a->kv_heads);
-  l.part = packed_splits(a->tk) || packed_splits(a->tq) ? part_floats(a->d) : 0;
+  l.part_q = packed_splits(a->tk) ? part_floats(a->d) : 0;
+  l.part = packed_splits(a->tq) ? part_floats(a->d) : 0;
   l.sum = l.splits > 1 ? (int64_t)l.splits * a->kv_heads * a->tk * a->d : 0;
   const int64_t of_q = plan_floats(a, a->tq, a->heads, a->tk), of_k = plan_floats(a, a->tk, a->kv_heads * l.splits, a->tq);
   l.plan = of_q > of_k ? of_q : of_k;   // (dq's is read before dk's is written)
-  l.bytes = (l.plan + kRecordFloats + l.delta + 2 * l.part + 2 * l.sum) * 4;
+  l.bytes = (l.plan + 2 * kRecordFloats + l.delta + l.part_q + 2 * l.part + 2 * l.sum) * 4;
   return l;
 }
 static bool sizes_ok(const vmo_packed_args* a) {
@@ -125,8 +126,9 @@ extern "C" int vmo_packed_bwd(const vmo_packed_args* a, void* stream) {
   p.splits = l.splits;
   if (l.plan > 0) p.plan = (i32x4*)a->workspace;
   p.records = (i32x4*)((float*)a->workspace + l.plan);
-  p.neg_delta = (float*)p.records + kRecordFloats;
-  p.part = p.neg_delta + l.delta;
+  p.neg_delta = (float*)p.records + 2 * kRecordFloats;   // (dk's and dv's records, then dq's)
+  p.part_q = p.neg_delta + l.delta;
+  p.part = p.part_q + l.part_q;
   p.part2 = p.part + l.part;
   p.sum = p.part2 + l.part;
   p.sum2 = p.sum + l.sum;

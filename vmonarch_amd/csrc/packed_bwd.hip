@@ -405,10 +405,11 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
 // dq, or dk and dv, of split tiles from their parts, in the parts' order: the workgroup of part k takes its share of the
 // tile's rows, D / 4 lanes a row, kJoinRows of them at a time.
 template <bool F16, int D, bool KEYS>
-__global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams p) {
+__device__ __forceinline__ void packed_bwd_join(const PackedParams& p) {
   using T = typename Elem<F16>::T;
   using V4 = typename Elem<F16>::V4;
   constexpr int TPR = D / 4, STEP = 256 / TPR;
+  if (p.split_least == 0) return;
   const i32x4 rec = p.records[blockIdx.x];   // first row, rows, part, parts
   if (rec[3] <= 1) return;
   const int shares = p.per, hs = packed_head(packed_place(p, blockIdx.x).pos, shares), parts = rec[3];
@@ -451,6 +452,13 @@ __global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams p) {
       }
     }
   }
+}
+
+// All of them in one launch: a launch that finds little to add takes 4 to 5 us.
+template <bool F16, int D>
+__global__ __launch_bounds__(256) void packed_bwd_join_kernel(PackedParams of_k, PackedParams of_q) {
+  if (blockIdx.y == 0) packed_bwd_join<F16, D, true>(of_k);
+  else packed_bwd_join<F16, D, false>(of_q);
 }
 
 // dk and dv from the sums of workgroups that had some of the group's heads each, in their order; rows outside every sequence
@@ -503,21 +511,19 @@ template <bool F16, int D>
 static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   constexpr int LDS_Q = packed_dq_lds<D>(), LDS_KV = packed_kv_lds<D>();
   static_assert(LDS_Q <= 65536 && LDS_KV <= 80 * 1024, "two workgroups a CU");
-  auto join = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3(kPackedParts), dim3(256), 0, s, p);
-    return launch_status("packed_bwd_join");
-  };
+  PackedParams q = p;   // dq's launch
+  q.records = p.records + kPackedParts;
+  q.part = p.part_q;
   int rc = VMO_OK;
   if (p.tq > 0) {
-    p.split_least = packed_splits(p.tk) ? kPackedSplit : 0;
-    rc = packed_begin<false>(&p, p.tq, p.heads, s);
+    q.split_least = packed_splits(p.tk) ? kPackedSplit : 0;
+    rc = packed_begin<false>(&q, p.tq, p.heads, s);
     if (rc != VMO_OK) return rc;
-    hipLaunchKernelGGL((packed_bwd_dq_kernel<F16, D>), dim3((unsigned)(p.blocks * p.per)), dim3(64 * kPackedWaves), LDS_Q, s, p);
+    hipLaunchKernelGGL((packed_bwd_dq_kernel<F16, D>), dim3((unsigned)(q.blocks * q.per)), dim3(64 * kPackedWaves), LDS_Q, s, q);
     rc = launch_status("packed_bwd_dq");
-    if (rc == VMO_OK && p.split_least > 0) rc = join(packed_bwd_join_kernel<F16, D, false>);
     if (rc != VMO_OK) return rc;
   }
-  if (p.tk == 0) return VMO_OK;
+  if (p.tk == 0) return VMO_OK;   // (no tile of dq's is split)
   auto kern = packed_bwd_dkdv_kernel<F16, D>;
   if (LDS_KV > 65536 &&
       hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_KV) != hipSuccess)
@@ -528,7 +534,10 @@ static int launch_packed_bwd(PackedParams p, hipStream_t s) {
   hipLaunchKernelGGL(kern, dim3((unsigned)(p.blocks * p.per)), dim3(64 * kPackedWaves), LDS_KV, s, p);
   rc = launch_status("packed_bwd_dkdv");
   if (rc != VMO_OK) return rc;
-  if (p.split_least > 0) rc = join(packed_bwd_join_kernel<F16, D, true>);
+  if (p.split_least > 0 || q.split_least > 0) {
+    hipLaunchKernelGGL((packed_bwd_join_kernel<F16, D>), dim3(kPackedParts, 2), dim3(256), 0, s, p, q);
+    rc = launch_status("packed_bwd_join");
+  }
   if (rc != VMO_OK || p.splits == 1) return rc;
   const int64_t threads = (int64_t)p.tk * (D / 4);
   hipLaunchKernelGGL((packed_bwd_sum_kernel<F16, D>), dim3((unsigned)((threads + 255) / 256), (unsigned)min(p.kv_heads, 65535)),
