@@ -35,6 +35,7 @@ struct PackedParams {
   int splits;                              // dk / dv: workgroups that share a key tile, each with group / splits of the heads
   int split_least;                         // tiles of up to so many units are never split (0: no tile is)
   float c, sm_scale;                       // c = sm_scale log2 e
+  int half;                                // kPackedSlots / 2 / per
   float* part_q;                           // the backward's launch: dq's parts (part, part2: dk's and dv's)
 };
 
@@ -93,12 +94,12 @@ __device__ __forceinline__ int packed_count(const PackedTiles& t, int level) {
 // faster than two that share it, so up to S a tile is no later than the rest --, or 6 above 1.25 times the mean where that is
 // less (long prompts, beside whose stages a part's own cost is small), and `split_least` at least; where the heaviest tile has
 // 1.25 S, those of L > S units are cut into ceil(L / S) parts of equal length.  One prompt of 16384 tokens, 2 heads of 128
-// over one: 248 -> 163 us; of 8192, 4 heads: 129 -> 92; 4 prompts of 20 to 5000, 4 heads: 85 -> 55.  Training steps of the
-// first two: 714 -> 677 and 405 -> 396 us against 1.75 times the mean everywhere; 1.25 times everywhere cost short batches (12
+// over one: 248 -> 153 us; of 8192, 4 heads: 129 -> 87; 4 prompts of 20 to 5000, 4 heads: 85 -> 51.  Training steps of the
+// first two: 658 -> 632 and 374 -> 370 us against 1.75 times the mean everywhere; 1.25 times everywhere cost short batches (12
 // prompts of 40 to 3900 keys, 12 heads: 75 -> 84 us).  Eight waves of two key groups instead, which halve every tile's time,
 // did less (176 and 99 -> 218 and 116).  Parts and whole tiles stand in one order, by their work, so the launch's last round
 // is made of light ones; as no part has less than half of S, all parts are among the first 2 kPackedSlots / 1.25 workgroups.
-// A part's fp32 sums go to slot = workgroup number; a second kernel adds them.
+// A part's fp32 sums go to slot = its number in that order times per + pos; a second kernel adds them.
 constexpr int kPackedSlots = 512;
 constexpr int kPackedParts = 2 * kPackedSlots + 128;
 constexpr int kJoinRows = 4;   // rows that a lane of an adding kernel has under way
@@ -130,6 +131,7 @@ struct PackedTile {
   PackedSeq s;
   int tile;           // of the sequence; below 0: none
   int part, parts;
+  int number;         // of the part, heaviest first
   int which, spare;   // of no tile: the spare workgroup's number, and how many there are
 };
 constexpr int kPackedSeqBytes = 16;   // LDS of a sequence while a wave finds its tile
@@ -146,7 +148,19 @@ __device__ __forceinline__ PackedPlace packed_place(const PackedParams& p, uint3
   return PackedPlace{(int)q, (int)r};
 }
 
-// The idx-th part over all sequences' tiles, heaviest tiles first (a tile's time is its keys, or queries: with the heavy ones
+// The part that the idx-th workgroups take.  The first `half` go to CUs of their own, the next ones beside them, in the same
+// order: so of the first 2 half, where all CUs have two, the second half is taken from its end, the lightest beside the
+// heaviest; where there are fewer parts than that, the CUs with two have the lightest.  (Training steps of one prompt of 16384
+// tokens, 2 heads of 128: 662 -> 632 us; of 8192, 4 heads: 385 -> 370; 12 prompts of 40 to 2900, 12 heads, in three rounds:
+// 68.5 -> 69.1.)
+__device__ __forceinline__ int packed_turn(int idx, int busy, int half) {
+  const int n = min(busy, 2 * half), two = n - half;
+  if (two <= 0 || idx >= n) return idx;
+  if (idx >= half) return n - 1 - (idx - half);
+  return idx < two ? idx + half - two : idx - two;
+}
+
+// The part in turn idx over all sequences' tiles, heaviest tiles first (a tile's time is its keys, or queries: with the heavy ones
 // first the chip's last round is made of light ones); p.per workgroups take each.  The largest level whose parts and those
 // above are more than idx is found by bisection over per-sequence counts, from rows and keys that lie in LDS (free again
 // after the call) if MANY, in the lanes else; a level holds the sequences in order.  Every wave of a workgroup calls it.
@@ -195,10 +209,12 @@ __device__ __forceinline__ PackedTile packed_locate(const PackedParams& p, int i
   r.tile = -1;
   r.part = 0;
   r.parts = 1;
+  r.number = idx;
   r.which = 0;
   r.spare = 1;
   int lo = 1, above = 0;   // the level, and the parts above it
   const int busy = total(1);
+  r.number = idx = packed_turn(idx, busy, p.half);
   bool found = idx < busy;
   if (found) {
     int hi = min(split.S, best) + 1;   // total(lo) > idx >= total(hi) = above
@@ -260,7 +276,7 @@ __global__ __launch_bounds__(64 * kPackedWaves) void packed_plan_kernel(PackedPa
   const PackedTile w = packed_locate<KEYS, true>(p, idx, (VMO_LDS int*)(VMO_LDS char*)smem_raw);
   if (idx < p.blocks && (threadIdx.x & 63) == 0) {
     p.plan[2 * idx] = i32x4{w.s.qb, w.s.nq, w.s.kb, w.s.nk};
-    p.plan[2 * idx + 1] = w.tile < 0 ? i32x4{-1, w.which, w.spare, 0} : i32x4{w.tile, w.part, w.parts, 0};
+    p.plan[2 * idx + 1] = w.tile < 0 ? i32x4{-1, w.which, w.spare, w.number} : i32x4{w.tile, w.part, w.parts, w.number};
   }
 }
 // this workgroup's tile
@@ -275,6 +291,7 @@ __device__ __forceinline__ PackedTile packed_tile(const PackedParams& p, int idx
   r.tile = t[0];
   r.part = t[0] < 0 ? 0 : t[1];
   r.parts = t[0] < 0 ? 1 : t[2];
+  r.number = t[3];
   r.which = t[1];
   r.spare = t[2];
   return r;
@@ -282,10 +299,10 @@ __device__ __forceinline__ PackedTile packed_tile(const PackedParams& p, int idx
 
 // What the adding kernel has to know of this workgroup's tile (rows of the side that the tile is of).
 template <bool KEYS>
-__device__ __forceinline__ void packed_record(const PackedParams& p, const PackedTile& w) {
-  if (p.split_least > 0 && blockIdx.x < kPackedParts && threadIdx.x == 0) {
+__device__ __forceinline__ void packed_record(const PackedParams& p, const PackedTile& w, int slot) {
+  if (p.split_least > 0 && slot < kPackedParts && threadIdx.x == 0) {
     const int first = w.tile * kPackedTile, rows = min(kPackedTile, (KEYS ? w.s.nk : w.s.nq) - first);
-    p.records[blockIdx.x] = i32x4{(KEYS ? w.s.kb : w.s.qb) + first, rows, w.part, w.tile < 0 ? 1 : w.parts};
+    p.records[slot] = i32x4{(KEYS ? w.s.kb : w.s.qb) + first, rows, w.part, w.tile < 0 ? 1 : w.parts};
   }
 }
 
@@ -405,6 +422,7 @@ inline int packed_begin(PackedParams* p, int rows, int per, hipStream_t s) {
   p->per = per;
   p->per_rcp = 0xffffffffu / (uint32_t)per;
   p->blocks = (int)packed_blocks(rows, p->n, per, p->split_least > 0);
+  p->half = kPackedSlots / 2 / per > 0 ? kPackedSlots / 2 / per : 1;
   if (!p->plan) return VMO_OK;
   hipLaunchKernelGGL((packed_plan_kernel<KEYS>), dim3((unsigned)((p->blocks + kPackedWaves - 1) / kPackedWaves)),
                      dim3(64 * kPackedWaves), (size_t)p->n * kPackedSeqBytes, s, *p);

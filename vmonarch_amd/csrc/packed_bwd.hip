@@ -55,7 +55,8 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
   const PackedPlace place = packed_place(p, blockIdx.x);
   const int head = uni(packed_head(place.pos, p.heads));
   const PackedTile w = packed_tile<false>(p, place.idx);
-  packed_record<false>(p, w);
+  const int slot_no = w.number * p.per + place.pos;
+  packed_record<false>(p, w, slot_no);
   if (w.tile < 0) {
     packed_zero_rest<T, D>((T*)p.dq + head * p.dq_sh, p.dq_sn, p.q_off, p.n, p.tq, w.which, w.spare);
     return;
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dq_kernel(Pac
   if (!live) return;
   VMO_LDS float* patch = (VMO_LDS float*)(smem + wave * kEpiPatchBytes);
   if (parts > 1) {
-    float* out = p.part + ((int64_t)blockIdx.x * kPackedTile + wave * 32) * D;
+    float* out = p.part + ((int64_t)slot_no * kPackedTile + wave * 32) * D;
     store_acc_rows<F16>(patch, acc, NA, p.sm_scale, kGradStoreF32, (char*)out, D * 4, min(32, nq - q0), lane);
     return;
   }
@@ -211,7 +212,8 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   const int hs = uni(packed_head(place.pos, p.per));
   const int kvh = hs / p.splits, split = hs % p.splits;
   const PackedTile w = packed_tile<true>(p, place.idx);
-  packed_record<true>(p, w);
+  const int slot_no = w.number * p.per + place.pos;
+  packed_record<true>(p, w, slot_no);
   if (w.tile < 0) {
     if (p.splits == 1) {
       packed_zero_rest<T, D>((T*)p.dk + kvh * p.dk_sh, p.dk_sn, p.k_off, p.n, p.tk, w.which, w.spare);
@@ -391,7 +393,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_bwd_dkdv_kernel(P
   const int nrows = min(32, nk - k0);
   if (parts > 1 || p.splits > 1) {
     const bool slot = parts > 1;
-    const int64_t r = (slot ? (int64_t)blockIdx.x * kPackedTile + wave * 32 : (int64_t)(split * p.kv_heads + kvh) * p.tk + kb + k0) * D;
+    const int64_t r = (slot ? (int64_t)slot_no * kPackedTile + wave * 32 : (int64_t)(split * p.kv_heads + kvh) * p.tk + kb + k0) * D;
     store_acc_rows<F16>(patch, dk, NA, p.sm_scale, kGradStoreF32, (char*)((slot ? p.part : p.sum) + r), D * 4, nrows, lane);
     store_acc_rows<F16>(patch, dv, NA, 1.0f, kGradStoreF32, (char*)((slot ? p.part2 : p.sum2) + r), D * 4, nrows, lane);
   } else {

@@ -47,7 +47,8 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
   const PackedPlace place = packed_place(p, blockIdx.x);
   const int head = uni(packed_head(place.pos, p.heads));
   const PackedTile w = packed_tile<false>(p, place.idx);
-  packed_record<false>(p, w);
+  const int slot_no = w.number * p.per + place.pos;
+  packed_record<false>(p, w, slot_no);
   if (w.tile < 0) {
     if (p.zero_rest)
       packed_zero_rest<T, D>((T*)p.out + head * p.o_sh, p.o_sn, p.q_off, p.n, p.tq, w.which, w.spare);
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(64 * kPackedWaves, 2) void packed_fwd_kernel(Packed
   const int nrows = min(32, nq - q0);
   VMO_LDS float* patch = (VMO_LDS float*)(smem + wave * kEpiPatchBytes);
   if (parts > 1) {
-    const int64_t at = (int64_t)blockIdx.x * kPackedTile + wave * 32;
+    const int64_t at = (int64_t)slot_no * kPackedTile + wave * 32;
     store_acc_rows<F16>(patch, acc, NA, 1.f, kGradStoreF32, (char*)(p.part + at * D), D * 4, nrows, lane);
     if (hl == 0 && l32 < nrows) {
       p.part2[2 * (at + l32)] = m_run;
