@@ -367,3 +367,17 @@ def test_scale_zero_is_the_mean(page):
     o = paged_attention(q, k, v, table, lens, sm_scale=0.0)
     for b in range(3):
         assert_within(o[b], want_one(q[b], rows[b], 0.0, torch.float16), f"sequence {b}")
+
+
+def test_several_new_tokens_of_one_sequence():
+    """A row each, all with the sequence's pages and lengths that grow: the prompt's attention after cached keys."""
+    from vmonarch_amd import paged_attention
+    g = torch.Generator().manual_seed(43)
+    past, new, H, D = 500, 70, 8, 128
+    k, v, table, lens, rows = cache(g, [past + new], 2, D, 16, torch.bfloat16)
+    q = torch.randn(new, H, D, generator=g).bfloat16().to(DEV)
+    lengths = torch.arange(past + 1, past + new + 1, device=DEV, dtype=torch.int32)
+    o = paged_attention(q, k, v, table.expand(new, -1), lengths)
+    for i in range(0, new, 3):
+        n = past + i + 1
+        assert_within(o[i], want_one(q[i], tuple(x[:, :n] for x in rows[0]), D ** -0.5, torch.bfloat16), f"token {i}")

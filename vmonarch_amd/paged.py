@@ -26,8 +26,9 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, sm_scale=None, out
     Returns:
         o: (B, H, D) in q's dtype; 0 for a sequence without tokens.
 
-    Table and lengths are read on the GPU when the kernels run (a captured graph replays with what they then hold).  A
-    page number outside the cache, or a length beyond W pages, is not followed: that sequence's rows are NaN.  Not
+    Several new tokens of one sequence are that many rows with its pages (one row of a table, expanded) and growing
+    lengths.  Table and lengths are read on the GPU when the kernels run (a captured graph replays with what they then hold).
+    A page number outside the cache, or a length beyond W pages, is not followed: that sequence's rows are NaN.  Not
     differentiable: where gradients are recorded the call is refused, as those below are.
     """
     if sm_scale is None:
