@@ -3,8 +3,8 @@
 A value is off by at most half a step of a rounding: u = eps / 2 of the 16-bit type, relative to it.  The forward rounds
 each weight P once (its operand of P V) and o once, so with A = P |v|
     |o - o*| <= u A + u |o*|.
-The backward rounds P (operand of dV), dS (operand of dQ and dK) and each gradient once; delta = rowsum(o dO) takes the
-rounded o, so it is off by at most e_i = sum_d |dO_id| u (A_id + |o_id|), and dS by P e:
+The backward rounds P (operand of dV), dS (operand of dQ and dK) and each gradient once; with an o as above delta =
+rowsum(o dO) is off by at most e_i = sum_d |dO_id| u (A_id + |o_id|) (less where it takes o before its rounding), and dS by P e:
     |dV - dV*| <= u P^T |dO| + u |dV*|,
     |dQ - dQ*| <= sm (u |dS| + P e) |K| + u |dQ*|,   |dK - dK*| <= sm (u |dS| + P e)^T |Q| + u |dK*|.
 32-bit arithmetic adds FP32 = 2^-16 of the sums of absolute values (weights: the exponent s c - m, of size up to 2^6 here,

@@ -355,3 +355,26 @@ def test_a_buffer_that_is_written_counts_as_changed():
     packed_attention(q, q, q, offsets([10]), out=out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_rows_far_apart():
+    """Tokens 2 MB apart, so a sequence's rows reach 6 GB from its first: bit for bit as rows beside each other."""
+    from vmonarch_amd import packed_attention
+    g = torch.Generator().manual_seed(23)
+    T, D = 3000, 64
+    buf = torch.empty(T, 1 << 20, device=DEV, dtype=torch.bfloat16)
+    near = [tensor(g, h, T, D, torch.bfloat16, "nhd") for h in (2, 1, 1, 2)]
+    far, at = [], 0
+    for t in near:
+        far.append(buf[:, at:at + t.shape[0] * D].view(T, t.shape[0], D).transpose(0, 1).copy_(t))
+        at += t.shape[0] * D
+    out = buf[:, at:at + 2 * D].view(T, 2, D).transpose(0, 1)
+    off = offsets([40, T - 40])
+    leaves = [[t.detach().requires_grad_() for t in x[:3]] for x in (near, far)]
+    want, got = (packed_attention(*x, off) for x in leaves)
+    assert torch.equal(want, got)
+    for a, b in zip(torch.autograd.grad(want, leaves[0], near[3]), torch.autograd.grad(got, leaves[1], far[3])):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        packed_attention(*far[:3], off, out=out)
+    assert torch.equal(want, out)
