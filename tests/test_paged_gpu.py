@@ -381,3 +381,25 @@ def test_several_new_tokens_of_one_sequence():
     for i in range(0, new, 3):
         n = past + i + 1
         assert_within(o[i], want_one(q[i], tuple(x[:, :n] for x in rows[0]), D ** -0.5, torch.bfloat16), f"token {i}")
+
+
+def test_in_inference_mode():
+    """A cache made outside or inside of it, and weights that would record gradients elsewhere."""
+    from vmonarch_amd import PagedKVCache, append_pages, packed_attention, paged_attention
+    g = torch.Generator().manual_seed(47)
+    q, k, v = (torch.randn(h, 60, 64, generator=g).bfloat16().to(DEV).requires_grad_() for h in (4, 2, 2))
+    off = torch.tensor([0, 45, 60], device=DEV, dtype=torch.int32)
+    outside = PagedKVCache(12, 16, 2, 64)
+    with torch.inference_mode():
+        want = packed_attention(q, k, v, off)
+        for cache_ in (outside, PagedKVCache(12, 16, 2, 64)):
+            ids = [cache_.open(), cache_.open()]
+            table, lengths = cache_.grow(ids, [45, 15])
+            append_pages(k, v, *cache_.layer(), table, lengths, off)
+            twin = cache_.fork(ids[0])
+            cache_.grow([twin])                            # copies the page that both would write
+            o = paged_attention(q[:, [44, 59]].transpose(0, 1), *cache_.layer(), *cache_.tables(ids))
+            for b, row in enumerate((44, 59)):
+                a, n = (0, 45) if b == 0 else (45, 15)
+                assert_within(o[b], want_one(q[:, row], (k[:, a:a + n], v[:, a:a + n]), 0.125, torch.bfloat16), f"sequence {b}")
+                assert_within(want[:, row], want_one(q[:, row], (k[:, a:a + n], v[:, a:a + n]), 0.125, torch.bfloat16), f"row {row}")
