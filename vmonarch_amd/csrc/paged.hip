@@ -439,19 +439,23 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 }
 
 // ------------------------------------------------------------------------------------------------
-constexpr int kCopyPairs = 448;   // page pairs of a launch: they travel as its argument (3.5 KB of 4 KB)
+// Page pairs of a launch travel as its argument, at most 3.5 of its 4 KB; up to 48 pairs a small one (0.2 us less of the 3.8 that
+// a call with one pair takes the host).
+constexpr int kCopyPairs = 448, kCopyFew = 48;
+template <int PAIRS>
 struct CopyParams {
   char *k, *v;
   int64_t page_bytes, layer_bytes;
-  int pairs, pieces;
-  int32_t src[kCopyPairs], dst[kCopyPairs];
+  int pieces;
+  int32_t src[PAIRS], dst[PAIRS];
 };
 constexpr int kCopyPiece = 256 * 16;   // bytes a workgroup moves
 
 // Pages src[i] to dst[i] of every layer, K and V.  Bound by memory (12 layers x 256 pages of 16 KB: 29.7 us, 6.8 TB/s, some of
 // it from the last-level cache), the small copies by the launch (32 pages: 4.1 us).  One 16-byte piece a lane: with four the
 // two were 9% and 29% slower (fewer workgroups start slower); stored past the caches: 15% on the small one.
-__global__ __launch_bounds__(256) void paged_copy_kernel(CopyParams p) {
+template <int PAIRS>
+__global__ __launch_bounds__(256) void paged_copy_kernel(CopyParams<PAIRS> p) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));   // (HIP's own uint4 went through registers one at a time)
   const int piece = (int)blockIdx.x % p.pieces, pair = (int)blockIdx.x / p.pieces, layer = (int)blockIdx.y;
   char* base = (blockIdx.z ? p.v : p.k) + layer * p.layer_bytes;
@@ -461,6 +465,19 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(CopyParams p) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------
+template <int PAIRS>
+static int launch_copy(const vmo_copy_args* a, int first, int pairs, int pieces, hipStream_t s) {
+  CopyParams<PAIRS> p;
+  p.k = (char*)a->k; p.v = (char*)a->v; p.page_bytes = a->page_bytes; p.layer_bytes = a->layer_bytes;
+  p.pieces = pieces;
+  for (int i = 0; i < PAIRS; ++i) {
+    p.src[i] = i < pairs ? a->src[first + i] : 0;
+    p.dst[i] = i < pairs ? a->dst[first + i] : 0;
+  }
+  hipLaunchKernelGGL((paged_copy_kernel<PAIRS>), dim3((unsigned)(pieces * pairs), (unsigned)a->layers, 2), dim3(256), 0, s, p);
+  return launch_status("copy_pages");
+}
+
 // Waves of a launch: as many as the chip holds at once (256 CUs of 160 KB LDS), one round.  LDS of a wave: two K and two V
 // tiles, four slots of its group's queries.
 struct PagedShape { int blocks, per, q_rows, lds, waves; };
@@ -614,17 +631,9 @@ extern "C" int vmo_copy_pages(const vmo_copy_args* a, void* stream) {
     return set_error(VMO_ERR_INVALID, "copy_pages: page %d to %d of %d (each below that, none written twice or written and read)",
                      a->src[at], a->dst[at], a->pages);
   for (int done = 0; done < a->pairs; done += kCopyPairs) {
-    CopyParams p{};
-    p.k = (char*)a->k; p.v = (char*)a->v; p.page_bytes = a->page_bytes; p.layer_bytes = a->layer_bytes;
-    p.pairs = a->pairs - done < kCopyPairs ? a->pairs - done : kCopyPairs;
-    p.pieces = (int)pieces;
-    for (int i = 0; i < p.pairs; ++i) {
-      p.src[i] = a->src[done + i];
-      p.dst[i] = a->dst[done + i];
-    }
-    hipLaunchKernelGGL(paged_copy_kernel, dim3((unsigned)(p.pieces * p.pairs), (unsigned)a->layers, 2), dim3(256), 0,
-                       (hipStream_t)stream, p);
-    const int rc = launch_status("copy_pages");
+    const int pairs = a->pairs - done < kCopyPairs ? a->pairs - done : kCopyPairs;
+    const int rc = pairs <= kCopyFew ? launch_copy<kCopyFew>(a, done, pairs, (int)pieces, (hipStream_t)stream)
+                                     : launch_copy<kCopyPairs>(a, done, pairs, (int)pieces, (hipStream_t)stream);
     if (rc != VMO_OK) return rc;
   }
   return VMO_OK;
